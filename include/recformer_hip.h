@@ -542,6 +542,38 @@ int rf_global_query_bwd(int dtype, int B, int Lp, int D, int gmax, const int32_t
                         float q_scale, const void* h, int ldh, const void* wqgT, float* dwqg, float* dbqg, void* dh,
                         int lddh, rf_stream_t stream);
 
+/* Log probabilities of given entries, the entropy and the k best alternatives of each row of a logits
+ * matrix (N items or words), beside rf_cross_entropy_fwd: with t = (x - max) * inv_temp,
+ * logp = t - ln sum e^t. logits: (M, N), row stride ldx elements, any alignment of the element type.
+ * tokens: (M, C) entries, C <= 1024; ignore_index gives 0, another id outside [0, N) NaN. logp: (M, C) fp32.
+ * entropy: (M) fp32 or NULL. top_logp / top_ids: (M, k), k <= min(N, 256), largest logit first, the lower
+ * index first among equals (NaN above +inf), or NULL with k = 0. stats: (M, 4) fp32 or NULL: what the
+ * backward reads. -inf logits are masked columns; a row of nothing else gives -inf, entropy 0, and the
+ * lowest indices. workspace: rf_logprobs_workspace bytes, 16-byte aligned (rf_topk_distill_fwd: k = 0). */
+size_t rf_logprobs_workspace(int dtype, int M, int N, int k);
+int rf_token_logprobs_fwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp,
+                          const int64_t* tokens, int C, int64_t ignore_index, int k, float* logp, float* entropy,
+                          float* top_logp, int64_t* top_ids, float* stats, void* workspace, rf_stream_t stream);
+/* Its gradient: dlogits (M, N), the logits' type, row stride ldd, rows aligned as the logits' rows
+ * (addresses equal modulo 16 bytes); g_logp (M, C) fp32 or NULL, g_entropy (M) fp32 or NULL (then with
+ * entropy). Rows that are all -inf get 0; a row with an id that is neither valid nor ignore_index NaN. */
+int rf_token_logprobs_bwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp,
+                          const float* stats, const int64_t* tokens, int C, int64_t ignore_index, const float* g_logp,
+                          const float* entropy, const float* g_entropy, void* dlogits, int64_t ldd,
+                          rf_stream_t stream);
+/* Distillation from a teacher's best logits: per row KL(q || p) with q = softmax(teacher * inv_temp) over the
+ * K <= 1024 listed ids (teacher (M, K) fp32, ids (M, K); id -1 or teacher -inf: slot not used) and p =
+ * softmax(logits * inv_temp) over all N. rows: (M) fp32 losses (0 for a row that uses no slot, NaN for one
+ * with another id outside [0, N)); stats (M, 4) fp32; loss / coef: one fp32 each or NULL: scale *
+ * sum(rows) / n and scale / n, n the rows that use a slot. The same id twice counts twice. Gradient: dlogits as above, of
+ * g[0] * coef[0] * sum(rows) (device scalars: the upstream gradient and coef). */
+int rf_topk_distill_fwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp, const float* teacher,
+                        const int64_t* ids, int K, float scale, float* rows, float* stats, float* loss,
+                        float* coef, void* workspace, rf_stream_t stream);
+int rf_topk_distill_bwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp, const float* stats,
+                        const float* teacher, const int64_t* ids, int K, const float* g, const float* coef,
+                        void* dlogits, int64_t ldd, rf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -126,6 +126,15 @@ SIGNATURES = {
     "rf_cross_entropy_fwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, P, ctypes.c_int64, P, P, P]),
     "rf_cross_entropy_bwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, P, ctypes.c_int64, P, P,
                                      ctypes.c_int64, P]),
+    "rf_logprobs_workspace": (ctypes.c_size_t, [c_int, c_int, c_int, c_int]),
+    "rf_token_logprobs_fwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, c_float, P, c_int, ctypes.c_int64, c_int,
+                                      P, P, P, P, P, P, P]),
+    "rf_token_logprobs_bwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, c_float, P, P, c_int, ctypes.c_int64, P,
+                                      P, P, P, ctypes.c_int64, P]),
+    "rf_topk_distill_fwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, c_float, P, P, c_int, c_float, P, P, P, P,
+                                    P, P]),
+    "rf_topk_distill_bwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, c_float, P, P, P, c_int, P, P, P,
+                                    ctypes.c_int64, P]),
 }
 
 _LIB: Optional[ctypes.CDLL] = None

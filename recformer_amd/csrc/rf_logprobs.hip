@@ -1,0 +1,773 @@
+// What the softmax of a logits row says and how it learns, beside the cross entropy of rf_rowops.hip:
+// log probabilities of given entries, the entropy, the k best alternatives, a teacher's best logits to
+// learn from, and the gradients of all of them. For a row x of N logits and an inverse temperature it,
+//
+//   m = max_c x_c,  t_c = (x_c - m) it,  s = sum_c e^t_c,  logp_c = t_c - ln s,  p_c = e^logp_c
+//   H = ln s - (sum_c e^t_c t_c) / s                        (both terms >= 0: nothing cancels)
+//   top k: the k largest x_c, the lower index first among equals
+//   distillation: q = softmax(teacher logits it) over the row's K listed ids (id -1 or logit -inf: not
+//     listed), loss = sum_k q_k (ln q_k - logp_id_k)
+//   gradients:  dx_c = it (a p_c + b p_c logp_c + sum of w_j over the listed entries j with id_j = c)
+//     log probabilities (weights g_j) and entropy (weight h): a = -sum_j g_j - h H, b = -h, w_j = g_j
+//     distillation (weight g): a = g (0 for a row that lists nothing), b = 0, w_j = -g q_j
+//
+// -inf logits (masked columns) have p = 0 and add nothing. A row that is all -inf has no distribution:
+// log probabilities -inf, entropy 0, gradient 0. NaN or +inf in a row makes its numbers NaN (its top ids
+// stay defined: NaN first). Entries equal to ignore_index count 0 and get no gradient; any other id
+// outside [0, N) makes its number NaN.
+//
+// HBM bound: the forward reads the row once, the backward reads it once and writes it once. A workgroup
+// holds its slice of a row in registers (R 16-byte chunks a thread), so the maximum, the sums and the
+// alternatives all come from one read, and no running rescale is needed. Sums and exponents are fp32.
+// Long rows, and rows too few to fill the chip, are cut into slices whose (m, s, sum e^t t) and k best
+// are joined by a second launch; no atomics on memory, so results do not depend on scheduling.
+#include "rf_common.h"
+
+#include <algorithm>
+
+namespace rf {
+
+constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
+constexpr float LP_NINF = -__builtin_inff();
+constexpr int LP_R = 8;         // 16-byte chunks of a row per thread
+constexpr int LP_KMAX = 256;    // alternatives
+constexpr int LP_CAP = 2048;    // candidates a selection holds
+constexpr int LP_LIST = 1024;   // given entries / teacher entries per row
+
+// ---- elements of a row -----------------------------------------------------------------------
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T> struct Row;
+template <> struct Row<float> {
+  static constexpr int V = 4;
+  static constexpr uint32_t FILL = 0xFF800000u;
+  static __device__ __forceinline__ float at(const u32x4& r, int e) { return __uint_as_float(r[e]); }
+};
+template <> struct Row<bf16> {
+  static constexpr int V = 8;
+  static constexpr uint32_t FILL = 0xFF80FF80u;
+  static __device__ __forceinline__ float at(const u32x4& r, int e) {
+    return __uint_as_float(e & 1 ? r[e >> 1] & 0xFFFF0000u : r[e >> 1] << 16);
+  }
+};
+template <> struct Row<f16> {
+  static constexpr int V = 8;
+  static constexpr uint32_t FILL = 0xFC00FC00u;
+  static __device__ __forceinline__ float at(const u32x4& r, int e) {
+    const uint32_t w = r[e >> 1];  // (a bit cast of the vector's element itself would read element 0)
+    return (float)__builtin_bit_cast(f16x2, w)[e & 1];
+  }
+};
+
+// A row starts `off` elements into its first aligned 16-byte chunk; chunk j holds the columns
+// [j V - off, j V - off + V). Chunks that reach over an end of the row are read element by element.
+template <typename T>
+__device__ __forceinline__ int row_off(const T* x) {
+  return (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* x, int64_t c0, int N) {
+  constexpr int V = Row<T>::V;
+  if (c0 >= 0 && c0 + V <= N) return *reinterpret_cast<const u32x4*>(x + c0);
+  T v[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = c0 + e >= 0 && c0 + e < N ? x[c0 + e] : from_f32<T>(LP_NINF);
+  u32x4 r;
+  __builtin_memcpy(&r, v, 16);
+  return r;
+}
+
+// order of the alternatives: larger key first; -0 = +0, NaN above +inf
+__device__ __forceinline__ uint32_t key_of(float v) {
+  if (v != v) return 0xFFFFFFFFu;
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  if (k == 0xFFFFFFFFu) return __builtin_nanf("");
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// (key, column) as one number: larger = earlier in the list
+__device__ __forceinline__ uint64_t entry_of(float v, uint32_t col) {
+  return (uint64_t)key_of(v) << 32 | (uint32_t)~col;
+}
+
+// ---- workgroup reductions ----------------------------------------------------------------------
+template <int TPB>
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = wave_max(v);
+  if (TPB == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < TPB / 64; ++w) v = fmaxf(v, red[w]);
+  return v;
+}
+template <int TPB>
+__device__ __forceinline__ void block_sum2(float& a, float& b, float* red) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if (TPB == 64) return;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = a;
+    red[16 + (threadIdx.x >> 6)] = b;
+  }
+  __syncthreads();
+  a = red[0];
+  b = red[16];
+#pragma unroll
+  for (int w = 1; w < TPB / 64; ++w) {
+    a += red[w];
+    b += red[16 + w];
+  }
+}
+
+// ---- the k best of a workgroup's entries -------------------------------------------------------
+struct SelectLds {
+  uint64_t cand[LP_CAP];
+  uint32_t key[1024];  // the threads' largest keys; the histogram of the exact search
+  int count;
+  uint32_t tau;
+  uint64_t prefix;
+  int rem, done;
+};
+
+// the upper 16 bits of the k-th largest of a wave's keys (0 where it holds fewer)
+template <int PER>
+__device__ __forceinline__ uint32_t upper_bits(const uint32_t (&g)[PER], int k) {
+  uint32_t tau = 0;
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = tau | 1u << bit;
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) cnt += __popcll(__ballot(g[i] >= c));
+    if (cnt >= k) tau = c;
+  }
+  return tau;
+}
+
+// Collects into s.cand the candidates for the k best of the entries that the threads hold, at least
+// min(k, n) of them and among them the k best, and returns how many. src.each(tau, f) calls f(entry) for
+// every entry of the calling thread whose key is >= tau, src.again(f) for all its entries; tmax: the
+// thread's largest value; nan: some value is NaN (the float compares of the short way would miss it).
+//
+// Short way: the k-th largest of the threads' maxima is a lower bound of the k-th largest entry (k threads
+// hold one at least as large), and few entries lie above it: G groups of threads let about
+// G ln(G / (G - k)) through (52 for k = 50, G = 1024; 56 for G = 256, which takes a quarter of the counting).
+// One wave finds the bound's upper 16 bits by counting with ballots. Only where more than LP_CAP entries
+// pass (many equal values, or the best all in few threads) an exact search over the 64-bit entries by
+// 8-bit digits follows; its threshold lets exactly min(k, n) through.
+template <int TPB, typename Src>
+__device__ __forceinline__ int select_candidates(const Src& src, float tmax, bool nan, int k, int64_t n, SelectLds& s) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  s.key[t] = key_of(tmax);
+  if (t == 0) {
+    s.count = 0;
+    s.tau = 0;
+  }
+  __syncthreads();
+  if (n > LP_CAP && !nan) {
+    if (t < 64) {
+      constexpr int PER = TPB / 64;
+      uint32_t g[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) g[i] = s.key[i * 64 + t];
+      uint32_t tau;
+      if (PER == 16 && k <= 64) {  // groups of four threads
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = max(max(g[i], g[i + 4 % PER]), max(g[i + 8 % PER], g[i + 12 % PER]));
+        tau = upper_bits(q, k);
+      } else {
+        tau = upper_bits(g, k);
+      }
+      if (t == 0) s.tau = tau;
+    }
+    __syncthreads();
+  }
+  auto take = [&](uint64_t e) {
+    const int at = atomicAdd(&s.count, 1);
+    if (at < LP_CAP) s.cand[at] = e;
+  };
+  if (!nan) {
+    src.each(n > LP_CAP ? s.tau : 0u, take);
+    __syncthreads();
+    const int c = s.count;
+    if (c <= LP_CAP) return c;
+  }
+  // exact: the digits of the k-th largest entry from the top; stops as soon as a digit's whole bin is taken
+  const int kk = (int)(n < k ? n : k);
+  uint64_t prefix = 0;
+  int rem = kk, shift = 64;
+  while (true) {
+    __syncthreads();
+    for (int i = t; i < 256; i += TPB) s.key[i] = 0;
+    __syncthreads();
+    src.again([&](uint64_t e) {
+      if (shift == 64 || (e >> shift) == prefix) atomicAdd(&s.key[(e >> (shift - 8)) & 255], 1u);
+    });
+    __syncthreads();
+    if (t == 0) {
+      int above = 0, d = 255;
+      while (d > 0 && above + (int)s.key[d] < rem) above += s.key[d--];
+      s.prefix = prefix << 8 | (uint64_t)d;
+      s.rem = rem - above;
+      s.done = (int)s.key[d] == rem - above;
+    }
+    __syncthreads();
+    prefix = s.prefix;
+    rem = s.rem;
+    shift -= 8;
+    if (s.done || shift == 0) break;
+  }
+  const uint64_t least = prefix << shift;
+  __syncthreads();
+  if (t == 0) s.count = 0;
+  __syncthreads();
+  src.again([&](uint64_t e) {
+    if (e >= least) take(e);
+  });
+  __syncthreads();
+  return min(s.count, LP_CAP);
+}
+
+// f(rank, entry) for the candidates in list order: entries are all different, so an entry's rank is the
+// number of larger ones
+template <int TPB, typename F>
+__device__ __forceinline__ void rank_candidates(const SelectLds& s, int c, int k, F f) {
+  for (int i = threadIdx.x; i < c; i += TPB) {
+    const uint64_t e = s.cand[i];
+    int r = 0;
+    for (int j = 0; j < c; ++j) r += s.cand[j] > e;
+    if (r < k) f(r, e);
+  }
+}
+
+// ---- what a finished row gives -----------------------------------------------------------------
+struct LpArgs {
+  int M, N, S, cps;          // rows, columns, slices per row, chunks per slice
+  int64_t ld;
+  float it, c2;              // inverse temperature; it log2(e)
+  const int64_t* ids;        // given entries (M, C), or the teacher's (M, K)
+  int nids;
+  int64_t ignore;
+  const float* tval;         // teacher logits (M, K); NULL: log probabilities
+  int k;                     // alternatives
+  float* logp;               // (M, C), or the distillation loss per row (M)
+  float* entropy;            // (M) or NULL
+  float* top_logp;           // (M, k)
+  int64_t* top_ids;
+  float* stats;              // (M, 4): m, 1 / s, teacher maximum, 1 / teacher sum
+  float* part;               // (M S, 4): m, s, sum e^t t log2(e), -
+  uint64_t* pent;            // (M S, k) entries, 0 = none
+};
+
+// m, s and h = sum e^t t log2(e) of row r are known to the whole workgroup
+template <int TPB, typename T>
+__device__ __forceinline__ void finish_row(const LpArgs& a, int r, const T* __restrict__ x, float m, float s, float h,
+                                           float* red) {
+  const int t = threadIdx.x;
+  const bool empty = s == 0.f;
+  const float ls = empty ? 0.f : __builtin_amdgcn_logf(s) * LP_LN2;
+  auto logp_at = [&](int64_t id) {
+    const float v = to_f32(x[id]);
+    return empty || v == LP_NINF ? (s != s ? s : LP_NINF) : (v - m) * a.it - ls;
+  };
+  float tm = 0.f, trs = 0.f;
+  if (a.tval) {
+    const int64_t* id = a.ids + (int64_t)r * a.nids;
+    const float* tv = a.tval + (int64_t)r * a.nids;
+    float mx = LP_NINF;
+    for (int j = t; j < a.nids; j += TPB)
+      if (id[j] != -1) mx = fmaxf(mx, tv[j]);
+    tm = block_max<TPB>(mx, red);
+    if (tm == LP_NINF) tm = 0.f;
+    float ts = 0.f, cross = 0.f;
+    for (int j = t; j < a.nids; j += TPB) {
+      if (id[j] == -1) continue;
+      const float tz = (tv[j] - tm) * a.it;
+      const float e = __builtin_amdgcn_exp2f(tz * LP_LOG2E);
+      ts += e;
+      // a teacher logit of -inf teaches nothing, whatever the student says
+      if (e != 0.f) cross += e * (tz - (id[j] >= 0 && id[j] < a.N ? logp_at(id[j]) : __builtin_nanf("")));
+    }
+    block_sum2<TPB>(ts, cross, red);
+    trs = ts == 0.f ? 0.f : 1.f / ts;
+    // sum q (tz - ln ts - logp) with q = e / ts
+    if (t == 0) a.logp[r] = ts == 0.f ? 0.f : cross * trs - __builtin_amdgcn_logf(ts) * LP_LN2;
+  } else {
+    for (int j = t; j < a.nids; j += TPB) {
+      const int64_t id = a.ids[(int64_t)r * a.nids + j];
+      a.logp[(int64_t)r * a.nids + j] =
+          id == a.ignore ? 0.f : id >= 0 && id < a.N ? logp_at(id) : __builtin_nanf("");
+    }
+    if (t == 0 && a.entropy) a.entropy[r] = empty ? 0.f : ls - h / s * LP_LN2;
+  }
+  if (t == 0 && a.stats) {
+    float* st = a.stats + (int64_t)r * 4;
+    st[0] = m;
+    st[1] = empty ? 0.f : 1.f / s;
+    st[2] = tm;
+    st[3] = trs;
+  }
+}
+
+template <int TPB>
+__device__ __forceinline__ void write_top(const LpArgs& a, int r, float m, float s, const SelectLds& sel, int c) {
+  const bool empty = s == 0.f;
+  const float ls = empty ? 0.f : __builtin_amdgcn_logf(s) * LP_LN2;
+  rank_candidates<TPB>(sel, c, a.k, [&](int rank, uint64_t e) {
+    const float v = value_of((uint32_t)(e >> 32));
+    const int64_t o = (int64_t)r * a.k + rank;
+    a.top_logp[o] = empty || v == LP_NINF ? (s != s ? s : LP_NINF) : (v - m) * a.it - ls;
+    a.top_ids[o] = (int64_t)(uint32_t)~(uint32_t)e;
+  });
+}
+
+// A slice of a row: the short way looks at the chunks a thread holds, the exact search reads the row again
+// (it is rare, and unrolled over the registers its code would crowd out the rest).
+template <typename T, int TPB>
+struct RowSrc {
+  const T* x;
+  u32x4* raw;
+  int j0, jn, off, N;  // the slice's chunks [j0, j0 + jn)
+  template <typename F>
+  __device__ __forceinline__ void each(uint32_t tau, F f) const {
+    constexpr int V = Row<T>::V;
+    // keys at or below -inf's: every column; otherwise an ordinary float compare
+    const bool all = tau <= 0x007FFFFFu;
+    const float lim = all ? LP_NINF : value_of(tau);
+#pragma unroll
+    for (int i = 0; i < LP_R; ++i) {
+      const int j = i * TPB + (int)threadIdx.x;
+      if (j < jn) {
+        asm volatile("" : "+v"(raw[i]));
+        float top = Row<T>::at(raw[i], 0);
+#pragma unroll
+        for (int e = 1; e < V; ++e) top = fmaxf(top, Row<T>::at(raw[i], e));
+        if (all || top >= lim) {
+          asm volatile("" : "+v"(raw[i]));
+          const int64_t c0 = (int64_t)(j0 + j) * V - off;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float v = Row<T>::at(raw[i], e);
+            if ((all || v >= lim) && c0 + e >= 0 && c0 + e < N) f(entry_of(v, (uint32_t)(c0 + e)));
+          }
+        }
+      }
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void again(F f) const {
+    constexpr int V = Row<T>::V;
+    const int64_t c1 = min((int64_t)(j0 + jn) * V - off, (int64_t)N);
+    for (int64_t c = max((int64_t)j0 * V - off, (int64_t)0) + threadIdx.x; c < c1; c += TPB)
+      f(entry_of(to_f32(x[c]), (uint32_t)c));
+  }
+};
+
+// ---- one slice of a row ------------------------------------------------------------------------
+template <typename T, int TPB, bool ENT, bool TOP>
+__global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a, const T* __restrict__ logits) {
+  constexpr int V = Row<T>::V;
+  __shared__ float red[32];
+  __shared__ SelectLds sel;
+  const int t = threadIdx.x;
+  const int r = blockIdx.x / a.S, sl = blockIdx.x % a.S;
+  const T* x = logits + (int64_t)r * a.ld;
+  const int off = row_off(x);
+  const int nch = (int)(((int64_t)a.N + off + V - 1) / V);
+  const int j0 = min(sl * a.cps, nch), jn = min(a.cps, nch - j0);
+  u32x4 raw[LP_R];
+#pragma unroll
+  for (int i = 0; i < LP_R; ++i) {
+    const int j = i * TPB + t;
+    if (j < jn) raw[i] = load_chunk(x, (int64_t)(j0 + j) * V - off, a.N);
+    else raw[i] = u32x4{Row<T>::FILL, Row<T>::FILL, Row<T>::FILL, Row<T>::FILL};
+  }
+  float tmax = LP_NINF;
+#pragma unroll
+  for (int i = 0; i < LP_R; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) tmax = fmaxf(tmax, Row<T>::at(raw[i], e));
+  float m = block_max<TPB>(tmax, red);
+  if (m == LP_NINF) m = 0.f;
+  // per element: subtract, scale, v_exp, one add, and for the entropy a clamp (so that 0 * -inf stays 0;
+  // e^t is 0 from 2^-150 on) and an fma
+  // (the empty asm keeps the values packed between the passes: unpacked they would not fit the registers)
+  float s = 0.f, h = 0.f;
+#pragma unroll
+  for (int i = 0; i < LP_R; ++i) {
+    if (i * TPB < jn) {
+      asm volatile("" : "+v"(raw[i]));
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float u = (Row<T>::at(raw[i], e) - m) * a.c2;
+        const float p = __builtin_amdgcn_exp2f(u);
+        s += p;
+        if (ENT) h = fmaf(p, fmaxf(u, -200.f), h);
+      }
+    }
+  }
+  block_sum2<TPB>(s, h, red);
+  if (a.S == 1) {
+    finish_row<TPB>(a, r, x, m, s, h, red);
+  } else if (t == 0) {
+    float* p = a.part + (int64_t)blockIdx.x * 4;
+    p[0] = s == 0.f ? LP_NINF : m;
+    p[1] = s;
+    p[2] = h;
+  }
+  if (TOP) {
+    const int64_t first = max((int64_t)j0 * V - off, (int64_t)0);
+    const int64_t n = max(min((int64_t)(j0 + jn) * V - off, (int64_t)a.N) - first, (int64_t)0);
+    const RowSrc<T, TPB> src{x, raw, j0, jn, off, a.N};
+    const int c = select_candidates<TPB>(src, tmax, s != s, a.k, n, sel);
+    if (a.S == 1) {
+      write_top<TPB>(a, r, m, s, sel, c);
+    } else {
+      uint64_t* o = a.pent + (int64_t)blockIdx.x * a.k;
+      rank_candidates<TPB>(sel, c, a.k, [&](int rank, uint64_t e) { o[rank] = e; });
+      for (int i = c + t; i < a.k; i += TPB) o[i] = 0;
+    }
+  }
+}
+
+// ---- the slices of a row joined ----------------------------------------------------------------
+template <int TPB>
+struct ListSrc {
+  const uint64_t* ent;
+  int n;
+  template <typename F>
+  __device__ __forceinline__ void each(uint32_t tau, F f) const {
+    for (int i = threadIdx.x; i < n; i += TPB) {
+      const uint64_t e = ent[i];
+      if (e != 0 && (uint32_t)(e >> 32) >= tau) f(e);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void again(F f) const { each(0u, f); }
+};
+
+template <typename T, int TPB, bool TOP>
+__global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __restrict__ logits) {
+  __shared__ float red[32];
+  __shared__ SelectLds sel;
+  const int t = threadIdx.x, r = blockIdx.x;
+  const float* part = a.part + (int64_t)r * a.S * 4;
+  float m = LP_NINF;
+  for (int i = t; i < a.S; i += TPB) m = fmaxf(m, part[4 * i]);
+  m = block_max<TPB>(m, red);
+  if (m == LP_NINF) m = 0.f;
+  float s = 0.f, h = 0.f;
+  for (int i = t; i < a.S; i += TPB) {
+    const float mi = part[4 * i], si = part[4 * i + 1];
+    if (si == 0.f) continue;  // a slice with nothing in it
+    const float d = (mi - m) * a.c2;  // the slice's exponents move by d: sum e^(u + d) (u + d)
+    const float f = __builtin_amdgcn_exp2f(d);
+    s = fmaf(si, f, s);
+    h = fmaf(f, fmaf(fmaxf(d, -200.f), si, part[4 * i + 2]), h);
+  }
+  block_sum2<TPB>(s, h, red);
+  finish_row<TPB>(a, r, logits + (int64_t)r * a.ld, m, s, h, red);
+  if (TOP) {
+    const ListSrc<TPB> src{a.pent + (int64_t)r * a.S * a.k, a.S * a.k};
+    uint64_t best = 0;
+    src.again([&](uint64_t e) { best = max(best, e); });
+    const float tmax = best ? value_of((uint32_t)(best >> 32)) : LP_NINF;
+    const int c = select_candidates<TPB>(src, tmax, false, a.k, (int64_t)a.S * a.k, sel);
+    write_top<TPB>(a, r, m, s, sel, c);
+  }
+}
+
+// ---- mean of the rows' losses over the rows that list something --------------------------------
+// loss = scale sum(rows) / n, coef = scale / n with n = #{r : 1 / teacher sum != 0}; one workgroup, so
+// the order of the sum is fixed (0 / 0 = NaN where no row lists anything, as the mean cross entropy has it)
+__global__ void __launch_bounds__(1024) k_rows_mean(int M, const float* __restrict__ rows,
+                                                    const float* __restrict__ stats, float scale,
+                                                    float* __restrict__ loss, float* __restrict__ coef) {
+  __shared__ float red[32];
+  float a = 0.f, n = 0.f;
+  for (int r = threadIdx.x; r < M; r += 1024) {
+    a += rows[r];
+    n += stats[4 * (int64_t)r + 3] != 0.f ? 1.f : 0.f;
+  }
+  block_sum2<1024>(a, n, red);
+  if (threadIdx.x == 0) {
+    *loss = a * scale / n;
+    *coef = scale / n;
+  }
+}
+
+// ---- gradients ---------------------------------------------------------------------------------
+constexpr int LB_R = 4, LB_TPB = 256;
+
+struct LpBwdArgs {
+  int M, N, S, cps;
+  int64_t ld, ldd;
+  float it, c2;
+  const int64_t* ids;
+  int nids;
+  int64_t ignore;
+  const float* tval;    // teacher logits; NULL: log probabilities
+  const float* g;       // (M, C) weights of the log probabilities, or one weight of the loss; may be NULL
+  const float* coef;    // distillation: a factor of that weight
+  const float* entropy; // (M), with g_ent
+  const float* g_ent;   // (M) weights of the entropy or NULL
+  const float* stats;   // (M, 4)
+};
+
+// One slice of a row: read, e^t / s, write. The listed entries are then written again by one thread each
+// (after a barrier; the first of equal ids adds all their weights in list order), so nothing is added
+// atomically.
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* __restrict__ logits,
+                                                         T* __restrict__ dlogits) {
+  constexpr int V = Row<T>::V;
+  __shared__ float red[32];
+  __shared__ int32_t sid[LP_LIST];
+  __shared__ float sw[LP_LIST];
+  const int t = threadIdx.x;
+  const int r = blockIdx.x / a.S, sl = blockIdx.x % a.S;
+  const T* x = logits + (int64_t)r * a.ld;
+  T* dx = dlogits + (int64_t)r * a.ldd;
+  const int off = row_off(x);  // dx starts as far into its chunk (checked by the caller)
+  const int nch = (int)(((int64_t)a.N + off + V - 1) / V);
+  const int j0 = min(sl * a.cps, nch), jn = min(a.cps, nch - j0);
+  u32x4 raw[LB_R];
+#pragma unroll
+  for (int i = 0; i < LB_R; ++i) {
+    const int j = i * LB_TPB + t;
+    if (j < jn) raw[i] = load_chunk(x, (int64_t)(j0 + j) * V - off, a.N);
+  }
+  const float m = a.stats[4 * (int64_t)r], rs = a.stats[4 * (int64_t)r + 1];
+  const bool empty = rs == 0.f;
+  const float nan = __builtin_nanf("");
+  float ca = 0.f, cb = 0.f;
+  if (a.tval) {
+    const float tm = a.stats[4 * (int64_t)r + 2], trs = a.stats[4 * (int64_t)r + 3];
+    const float g = a.g[0] * a.coef[0];
+    float bad = 0.f, unused = 0.f;
+    for (int j = t; j < a.nids; j += LB_TPB) {
+      const int64_t id = a.ids[(int64_t)r * a.nids + j];
+      const float q = id == -1 ? 0.f : __builtin_amdgcn_exp2f((a.tval[(int64_t)r * a.nids + j] - tm) * a.c2) * trs;
+      const bool in = id >= 0 && id < a.N;
+      if (!in && id != -1 && q != 0.f) bad = nan;
+      sid[j] = in && q != 0.f ? (int32_t)id : -1;
+      sw[j] = -g * q;
+    }
+    block_sum2<LB_TPB>(bad, unused, red);
+    ca = trs == 0.f ? 0.f : g + bad;
+  } else {
+    float sum = 0.f, unused = 0.f;
+    for (int j = t; j < a.nids; j += LB_TPB) {
+      const int64_t id = a.ids[(int64_t)r * a.nids + j];
+      const bool in = id >= 0 && id < a.N;
+      const float g = a.g && id != a.ignore ? a.g[(int64_t)r * a.nids + j] : 0.f;
+      sum += in || id == a.ignore ? (id == a.ignore ? 0.f : g) : nan;
+      sid[j] = in && id != a.ignore ? (int32_t)id : -1;
+      sw[j] = g;
+    }
+    block_sum2<LB_TPB>(sum, unused, red);
+    ca = -sum;
+    if (ENT) {
+      cb = -a.g_ent[r];
+      ca = fmaf(cb, a.entropy[r], ca);
+    }
+  }
+  const float k1 = empty ? 0.f : a.it * rs;
+  const float lrs = empty ? 0.f : __builtin_amdgcn_logf(rs) * LP_LN2;  // -ln s
+  auto grad = [&](float v) {
+    const float u = (v - m) * a.c2;
+    const float c = ENT ? fmaf(cb, fmaf(fmaxf(u, -200.f), LP_LN2, lrs), ca) : ca;
+    return __builtin_amdgcn_exp2f(u) * (k1 * c);
+  };
+#pragma unroll
+  for (int i = 0; i < LB_R; ++i) {
+    const int j = i * LB_TPB + t;
+    if (j < jn) {
+      const int64_t c0 = (int64_t)(j0 + j) * V - off;
+      T o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = from_f32<T>(empty ? 0.f : grad(Row<T>::at(raw[i], e)));
+      if (c0 >= 0 && c0 + V <= a.N) {
+        u32x4 w;
+        __builtin_memcpy(&w, o, 16);
+        *reinterpret_cast<u32x4*>(dx + c0) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c0 + e >= 0 && c0 + e < a.N) dx[c0 + e] = o[e];
+      }
+    }
+  }
+  if (empty) return;
+  __syncthreads();
+  const int64_t first = (int64_t)j0 * V - off, last = (int64_t)(j0 + jn) * V - off;
+  for (int j = t; j < a.nids; j += LB_TPB) {
+    const int32_t id = sid[j];
+    if (id < 0 || id < first || id >= last) continue;
+    float w = 0.f;
+    bool head = true;
+    for (int i = 0; i < a.nids; ++i)
+      if (sid[i] == id) {
+        head &= i >= j;
+        w += sw[i];
+      }
+    if (head) dx[id] = from_f32<T>(fmaf(a.it, w, grad(to_f32(x[id]))));
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+static int lp_vec(int dtype) { return dtype == RF_F32 ? 4 : 8; }
+
+// Slices per row and chunks per slice. A slice is at most what a 1024-thread workgroup holds. Fewer rows
+// than two workgroups a CU are cut further, down to LP_MIN_CHUNKS chunks (8 KB, two chunks a thread of a
+// 256-thread workgroup), as long as the lists that the join reads stay within 16 entries a thread.
+constexpr int LP_CUS = 256, LP_MIN_CHUNKS = 512;
+static void lp_plan(int dtype, int M, int N, int k, int* S, int* cps) {
+  const int V = lp_vec(dtype);
+  const int64_t nch = ((int64_t)N + 2 * V - 2) / V;  // of a row that starts anywhere in a chunk
+  int64_t s = (nch + 1024 * LP_R - 1) / (1024 * LP_R);
+  const int64_t want = std::min({(int64_t)(2 * LP_CUS + M - 1) / M, nch / LP_MIN_CHUNKS,
+                                 (int64_t)16384 / std::max(k, 16)});
+  s = std::max(s, want);
+  s = std::max<int64_t>(s, 1);
+  *cps = (int)((nch + s - 1) / s);
+  *S = (int)((nch + *cps - 1) / *cps);
+}
+
+template <typename T, bool ENT, bool TOP>
+static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
+  const T* p = (const T*)x;
+  const unsigned grid = (unsigned)((int64_t)a.M * a.S);
+  if (a.cps <= 256 * LP_R) k_logprobs<T, 256, ENT, TOP><<<grid, 256, 0, st>>>(a, p);
+  else k_logprobs<T, 1024, ENT, TOP><<<grid, 1024, 0, st>>>(a, p);
+  if (a.S > 1) {
+    if (!TOP || a.S * a.k <= 2048) k_logprobs_join<T, 256, TOP><<<a.M, 256, 0, st>>>(a, p);
+    else k_logprobs_join<T, 1024, TOP><<<a.M, 1024, 0, st>>>(a, p);
+  }
+}
+
+static int lp_forward(const char* name, int dtype, const LpArgs& in, const void* logits, void* ws, hipStream_t st) {
+  LpArgs a = in;
+  RF_REQUIRE(dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16, "%s: bad dtype %d", name, dtype);
+  RF_REQUIRE(a.M >= 0 && a.N > 0 && a.ld >= a.N, "%s: bad shape M=%d N=%d ld=%lld", name, a.M, a.N, (long long)a.ld);
+  RF_REQUIRE(a.it > 0.f && a.it <= 3e38f, "%s: inverse temperature %g must be positive and finite", name, a.it);
+  RF_REQUIRE(a.nids >= 0 && a.nids <= LP_LIST, "%s: %d entries per row (0 to %d)", name, a.nids, LP_LIST);
+  RF_REQUIRE(a.k >= 0 && a.k <= LP_KMAX && a.k <= a.N, "%s: k=%d must be in [0, min(N, %d)]", name, a.k, LP_KMAX);
+  if (a.M == 0) return RF_OK;
+  RF_REQUIRE(logits && (a.nids == 0 || (a.ids && a.logp)) && (a.k == 0 || (a.top_logp && a.top_ids)),
+             "%s: null pointer", name);
+  RF_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == RF_F32 ? 3 : 1)) == 0, "%s: misaligned logits", name);
+  lp_plan(dtype, a.M, a.N, a.k, &a.S, &a.cps);
+  RF_REQUIRE((int64_t)a.M * a.S < 0x7FFFFFFF, "%s: %d rows of %d slices are too many", name, a.M, a.S);
+  if (a.S > 1) {
+    RF_REQUIRE(ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0, "%s: workspace missing or not 16-byte aligned", name);
+    a.part = (float*)ws;
+    a.pent = (uint64_t*)((char*)ws + (size_t)a.M * a.S * 16);
+  }
+  const bool ent = a.entropy != nullptr, top = a.k > 0;
+#define LP_T(T)                                                 \
+  if (ent && top) lp_launch<T, true, true>(a, logits, st);      \
+  else if (ent) lp_launch<T, true, false>(a, logits, st);       \
+  else if (top) lp_launch<T, false, true>(a, logits, st);       \
+  else lp_launch<T, false, false>(a, logits, st)
+  if (dtype == RF_F32) { LP_T(float); }
+  else if (dtype == RF_BF16) { LP_T(bf16); }
+  else { LP_T(f16); }
+#undef LP_T
+  RF_LAUNCH_CHECK(name);
+}
+
+static int lp_backward(const char* name, int dtype, const LpBwdArgs& in, const void* logits, void* dlogits,
+                       hipStream_t st) {
+  LpBwdArgs a = in;
+  RF_REQUIRE(dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16, "%s: bad dtype %d", name, dtype);
+  RF_REQUIRE(a.M >= 0 && a.N > 0 && a.ld >= a.N && a.ldd >= a.N, "%s: bad shape", name);
+  RF_REQUIRE(a.it > 0.f && a.it <= 3e38f, "%s: inverse temperature %g must be positive and finite", name, a.it);
+  RF_REQUIRE(a.nids >= 0 && a.nids <= LP_LIST, "%s: %d entries per row (0 to %d)", name, a.nids, LP_LIST);
+  if (a.M == 0) return RF_OK;
+  RF_REQUIRE(logits && dlogits && a.stats && (a.nids == 0 || a.ids), "%s: null pointer", name);
+  const int V = lp_vec(dtype), es = dtype == RF_F32 ? 4 : 2;
+  RF_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (es - 1)) == 0 &&
+                 ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) & 15) == 0 &&
+                 (a.ld - a.ldd) % V == 0,
+             "%s: the gradient's rows must be aligned as the logits' rows are", name);
+  const int64_t nch = ((int64_t)a.N + 2 * V - 2) / V;
+  a.S = (int)((nch + LB_TPB * LB_R - 1) / (LB_TPB * LB_R));
+  a.cps = (int)((nch + a.S - 1) / a.S);
+  RF_REQUIRE((int64_t)a.M * a.S < 0x7FFFFFFF, "%s: %d rows of %d slices are too many", name, a.M, a.S);
+  const unsigned grid = (unsigned)((int64_t)a.M * a.S);
+#define LB_T(T)                                                                                        \
+  if (a.g_ent) k_logprobs_bwd<T, true><<<grid, LB_TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits);       \
+  else k_logprobs_bwd<T, false><<<grid, LB_TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits)
+  if (dtype == RF_F32) { LB_T(float); }
+  else if (dtype == RF_BF16) { LB_T(bf16); }
+  else { LB_T(f16); }
+#undef LB_T
+  RF_LAUNCH_CHECK(name);
+}
+
+}  // namespace rf
+
+using namespace rf;
+
+extern "C" size_t rf_logprobs_workspace(int dtype, int M, int N, int k) {
+  if (M <= 0 || N <= 0 || k < 0) return 0;
+  int S, cps;
+  lp_plan(dtype, M, N, k, &S, &cps);
+  return S > 1 ? (size_t)M * S * (16 + 8 * (size_t)k) : 0;
+}
+
+extern "C" int rf_token_logprobs_fwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp,
+                                     const int64_t* tokens, int C, int64_t ignore_index, int k, float* logp,
+                                     float* entropy, float* top_logp, int64_t* top_ids, float* stats, void* workspace,
+                                     rf_stream_t stream) {
+  LpArgs a{};
+  a.M = M; a.N = N; a.ld = ldx; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.ids = tokens; a.nids = C; a.ignore = ignore_index; a.k = k;
+  a.logp = logp; a.entropy = entropy; a.top_logp = top_logp; a.top_ids = top_ids; a.stats = stats;
+  return lp_forward("rf_token_logprobs_fwd", dtype, a, logits, workspace, as_stream(stream));
+}
+
+extern "C" int rf_token_logprobs_bwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp,
+                                     const float* stats, const int64_t* tokens, int C, int64_t ignore_index,
+                                     const float* g_logp, const float* entropy, const float* g_entropy, void* dlogits,
+                                     int64_t ldd, rf_stream_t stream) {
+  RF_REQUIRE(!g_entropy || entropy, "rf_token_logprobs_bwd: the entropy's gradient needs the entropy");
+  LpBwdArgs a{};
+  a.M = M; a.N = N; a.ld = ldx; a.ldd = ldd; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.ids = tokens; a.nids = C; a.ignore = ignore_index; a.g = g_logp; a.entropy = entropy; a.g_ent = g_entropy;
+  a.stats = stats;
+  return lp_backward("rf_token_logprobs_bwd", dtype, a, logits, dlogits, as_stream(stream));
+}
+
+extern "C" int rf_topk_distill_fwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp,
+                                   const float* teacher, const int64_t* ids, int K, float scale, float* rows,
+                                   float* stats, float* loss, float* coef, void* workspace, rf_stream_t stream) {
+  RF_REQUIRE(K >= 1, "rf_topk_distill_fwd: K=%d teacher entries", K);
+  RF_REQUIRE(M <= 0 || (teacher && rows && stats), "rf_topk_distill_fwd: null pointer");
+  RF_REQUIRE(!loss == !coef, "rf_topk_distill_fwd: loss and coef go together");
+  LpArgs a{};
+  a.M = M; a.N = N; a.ld = ldx; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.ids = ids; a.nids = K; a.tval = teacher; a.logp = rows; a.stats = stats;
+  const int rc = lp_forward("rf_topk_distill_fwd", dtype, a, logits, workspace, as_stream(stream));
+  if (rc != RF_OK || !loss) return rc;
+  k_rows_mean<<<1, 1024, 0, as_stream(stream)>>>(M, rows, stats, scale, loss, coef);
+  RF_LAUNCH_CHECK("rf_topk_distill_fwd");
+}
+
+extern "C" int rf_topk_distill_bwd(int dtype, int M, int N, const void* logits, int64_t ldx, float inv_temp,
+                                   const float* stats, const float* teacher, const int64_t* ids, int K, const float* g,
+                                   const float* coef, void* dlogits, int64_t ldd, rf_stream_t stream) {
+  RF_REQUIRE(K >= 1, "rf_topk_distill_bwd: K=%d teacher entries", K);
+  RF_REQUIRE(M <= 0 || (teacher && g && coef), "rf_topk_distill_bwd: null pointer");
+  LpBwdArgs a{};
+  a.M = M; a.N = N; a.ld = ldx; a.ldd = ldd; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.ids = ids; a.nids = K; a.tval = teacher; a.g = g; a.coef = coef; a.stats = stats;
+  return lp_backward("rf_topk_distill_bwd", dtype, a, logits, dlogits, as_stream(stream));
+}

@@ -7,7 +7,8 @@ allocated by PyTorch's caching allocator; the library never allocates or syncs.
 from __future__ import annotations
 
 import contextlib
-from typing import Dict, List, Optional, Tuple
+import math
+from typing import Dict, List, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -22,6 +23,7 @@ __all__ = [
     "global_attention", "gather_global_rows", "row_inv_norm", "cos_scores", "cos_scores_cand",
     "cross_entropy",
     "cos_scores_bwd",
+    "TokenLogprobs", "token_logprobs", "token_logprobs_bwd", "topk_distill", "topk_distill_bwd",
     "RF_EPI_NONE", "RF_EPI_BIAS", "RF_EPI_BIAS_GELU", "RF_EPI_BIAS_GELU_AUX", "RF_EPI_BIAS_RESID", "RF_EPI_COS",
     "RF_EPI_DGELU",
 ]
@@ -971,3 +973,178 @@ def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int 
     if want_argmax:
         return loss, amax.to(torch.int64)
     return loss
+
+
+# ---- log probabilities, alternatives and distillation (rf_logprobs.hip) -----------------------------
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' answer. logp: as tokens, fp32; entropy (M,) or None; top_logp / top_ids (M, k) fp32 /
+    int64 or None; stats (M, 4) fp32: what token_logprobs_bwd reads."""
+
+    logp: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    top_logp: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+    stats: Optional[torch.Tensor]
+
+
+def _run(fn, what: str, ref: torch.Tensor, *args) -> None:
+    """fn(*args, stream) on ref's device (made current for the call where it is not) and its current stream."""
+    if ref.device.index == torch.cuda.current_device():
+        check(fn(*args, _stream(ref)), what)
+    else:
+        with torch.cuda.device(ref.device):
+            check(fn(*args, _stream(ref)), what)
+
+
+def _logit_rows(what: str, logits: torch.Tensor, inv_temp: float) -> int:
+    """Checks a (M, N) row-major view and the inverse temperature; its row stride."""
+    _dev(logits)
+    dtype_code(logits.dtype)
+    ld = _rowmajor(logits, "logits")
+    M, N = logits.shape
+    if N < 1 or N >= 2 ** 31 - 16 or M >= 2 ** 31:
+        raise ValueError(f"{what}: logits {tuple(logits.shape)}")
+    if M > 1 and ld < N:
+        raise ValueError(f"{what}: rows of the logits overlap (stride {ld} < {N})")
+    if not (inv_temp > 0 and math.isfinite(inv_temp)):
+        raise ValueError(f"{what}: inverse temperature {inv_temp} must be positive and finite")
+    return max(ld, N)
+
+
+def _row_list(what: str, t: torch.Tensor, logits: torch.Tensor, dtype=None) -> torch.Tensor:
+    """A contiguous (M, C) list beside the logits' rows: int64 ids, or values in `dtype`."""
+    if t.device != logits.device:
+        raise ValueError(f"{what}: on {t.device}, logits on {logits.device}")
+    if dtype is None and t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: int64 or int32 ids, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != logits.shape[0] or t.shape[1] > 1024:
+        raise ValueError(f"{what}: shape {tuple(t.shape)} for {logits.shape[0]} rows (up to 1024 entries each)")
+    return t.to(dtype or torch.int64).contiguous()
+
+
+def _like_rows(logits: torch.Tensor, ld: int) -> Tuple[torch.Tensor, int]:
+    """An empty (M, N) tensor whose rows are aligned as the logits' rows are (contiguous where theirs allow it)."""
+    M, N = logits.shape
+    es = logits.element_size()
+    v = 16 // es
+    ldd = N + (ld - N) % v
+    off = logits.data_ptr() % 16 // es
+    if off == 0 and ldd == N:
+        return torch.empty(M, N, dtype=logits.dtype, device=logits.device), ldd
+    buf = torch.empty(off + M * ldd, dtype=logits.dtype, device=logits.device)
+    return buf.as_strided((M, N), (ldd, 1), off), ldd
+
+
+def _logprobs_ws(lib, logits: torch.Tensor, k: int) -> Optional[torch.Tensor]:
+    n = lib.rf_logprobs_workspace(dtype_code(logits.dtype), logits.shape[0], logits.shape[1], k)
+    return torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, k: int = 0, inv_temp: float = 1.0,
+                   ignore_index: int = -100, want_entropy: bool = False, want_stats: bool = False) -> TokenLogprobs:
+    """Log probabilities under softmax(logits * inv_temp) of each row of a (M, N) bf16 / fp16 / fp32 view
+    (rf_token_logprobs_fwd): of the given tokens ((M,) or (M, C) ids, C <= 1024; ignore_index gives 0, any
+    other id outside [0, N) NaN), the entropy, and the k <= 256 best alternatives (largest logit first, the
+    lower id first among equals). Masked columns are -inf; a row of nothing else gives -inf, entropy 0."""
+    lib = _lib.load()
+    ld = _logit_rows("token_logprobs", logits, inv_temp)
+    M, N = logits.shape
+    if not 0 <= k <= min(N, 256):
+        raise ValueError(f"token_logprobs: k={k} must be in [0, min(N, 256)]")
+    ids = logp = None
+    C = 0
+    if tokens is not None:
+        ids = _row_list("token_logprobs: tokens", tokens.unsqueeze(1) if tokens.dim() == 1 else tokens, logits)
+        C = ids.shape[1]
+        logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+    elif not (k or want_entropy or want_stats):
+        raise ValueError("token_logprobs: no output requested")
+    dev = logits.device
+    ent = torch.empty(M, dtype=torch.float32, device=dev) if want_entropy else None
+    tv = torch.empty(M, k, dtype=torch.float32, device=dev) if k else None
+    ti = torch.empty(M, k, dtype=torch.int64, device=dev) if k else None
+    stats = torch.empty(M, 4, dtype=torch.float32, device=dev) if want_stats else None
+    ws = _logprobs_ws(lib, logits, k)
+    _run(lib.rf_token_logprobs_fwd, "rf_token_logprobs_fwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
+         float(inv_temp), _p(ids), C, int(ignore_index), k, _p(logp), _p(ent), _p(tv), _p(ti), _p(stats), _p(ws))
+    return TokenLogprobs(logp, ent, tv, ti, stats)
+
+
+def token_logprobs_bwd(logits: torch.Tensor, stats: torch.Tensor, tokens: Optional[torch.Tensor],
+                       g_logp: Optional[torch.Tensor], entropy: Optional[torch.Tensor] = None,
+                       g_entropy: Optional[torch.Tensor] = None, inv_temp: float = 1.0,
+                       ignore_index: int = -100) -> torch.Tensor:
+    """rf_token_logprobs_bwd: d(sum g_logp logp + sum g_entropy H) / d(logits) in the logits' type, from the
+    forward's stats (and its entropy, with g_entropy)."""
+    lib = _lib.load()
+    ld = _logit_rows("token_logprobs_bwd", logits, inv_temp)
+    M, N = logits.shape
+    f32 = torch.float32
+    ids, C = None, 0
+    if tokens is not None and g_logp is not None:
+        if g_logp.shape != tokens.shape:
+            raise ValueError(f"token_logprobs_bwd: g_logp {tuple(g_logp.shape)} for tokens {tuple(tokens.shape)}")
+        ids = _row_list("token_logprobs_bwd: tokens", tokens.reshape(M, -1) if M else tokens.reshape(0, 1), logits)
+        C = ids.shape[1]
+        g_logp = _row_list("token_logprobs_bwd: g_logp", g_logp.reshape(ids.shape), logits, f32)
+    if g_entropy is not None:
+        for t in (g_entropy, entropy):
+            if t is None or tuple(t.shape) != (M,) or t.device != logits.device:
+                raise ValueError("token_logprobs_bwd: entropy and g_entropy are (M,) beside the logits")
+        g_entropy, entropy = g_entropy.to(f32).contiguous(), entropy.to(f32).contiguous()
+    if tuple(stats.shape) != (M, 4) or stats.dtype != f32 or not stats.is_contiguous() or stats.device != logits.device:
+        raise ValueError("token_logprobs_bwd: stats is the forward's (M, 4) fp32")
+    out, ldd = _like_rows(logits, ld)
+    _run(lib.rf_token_logprobs_bwd, "rf_token_logprobs_bwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
+         float(inv_temp), _p(stats), _p(ids), C, int(ignore_index), _p(g_logp) if C else None, _p(entropy),
+         _p(g_entropy), _p(out), ldd)
+    return out
+
+
+def _teacher(what: str, logits, teacher_logits, teacher_ids):
+    ids = _row_list(f"{what}: teacher_ids", teacher_ids, logits)
+    val = _row_list(f"{what}: teacher_logits", teacher_logits, logits, torch.float32)
+    if ids.shape != val.shape or ids.shape[1] < 1:
+        raise ValueError(f"{what}: teacher_logits {tuple(val.shape)} for teacher_ids {tuple(ids.shape)}")
+    return val, ids
+
+
+def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor, inv_temp: float = 1.0,
+                 scale: float = 1.0):
+    """rf_topk_distill_fwd: per row KL(q || p), q = softmax(teacher_logits * inv_temp) over the listed
+    teacher_ids ((M, K <= 1024); id -1 or logit -inf: slot not used), p = softmax(logits * inv_temp) over all
+    columns. Returns (rows (M,), stats (M, 4), loss, coef): loss = scale * sum(rows) / n and coef = scale / n,
+    one-element device tensors, with n the rows that use a slot (nan if none does). teacher_logits may be log probabilities."""
+    lib = _lib.load()
+    ld = _logit_rows("topk_distill", logits, inv_temp)
+    M, N = logits.shape
+    val, ids = _teacher("topk_distill", logits, teacher_logits, teacher_ids)
+    dev = logits.device
+    rows = torch.empty(M, dtype=torch.float32, device=dev)
+    stats = torch.empty(M, 4, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    coef = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _logprobs_ws(lib, logits, 0)
+    _run(lib.rf_topk_distill_fwd, "rf_topk_distill_fwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
+         float(inv_temp), _p(val), _p(ids), ids.shape[1], float(scale), _p(rows), _p(stats), _p(loss), _p(coef), _p(ws))
+    return rows, stats, loss, coef
+
+
+def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: torch.Tensor,
+                     teacher_ids: torch.Tensor, g: torch.Tensor, coef: torch.Tensor,
+                     inv_temp: float = 1.0) -> torch.Tensor:
+    """rf_topk_distill_bwd: the gradient of g * coef * sum(rows) in the logits' type; g and coef one-element
+    fp32 device tensors (the upstream gradient and the forward's coef)."""
+    lib = _lib.load()
+    ld = _logit_rows("topk_distill_bwd", logits, inv_temp)
+    M, N = logits.shape
+    val, ids = _teacher("topk_distill_bwd", logits, teacher_logits, teacher_ids)
+    if tuple(stats.shape) != (M, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError("topk_distill_bwd: stats is the forward's (M, 4) fp32")
+    for t in (g, coef):
+        if t.numel() != 1 or t.dtype != torch.float32 or t.device != logits.device:
+            raise ValueError("topk_distill_bwd: g and coef are one-element fp32 tensors beside the logits")
+    out, ldd = _like_rows(logits, ld)
+    _run(lib.rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
+         float(inv_temp), _p(stats), _p(val), _p(ids), ids.shape[1], _p(g), _p(coef), _p(out), ldd)
+    return out

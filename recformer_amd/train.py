@@ -44,7 +44,7 @@ import torch.nn.functional as F
 
 from . import dropout, ops
 
-__all__ = ["encode_train", "cos_scores_train", "cross_entropy_train"]
+__all__ = ["encode_train", "cos_scores_train", "cross_entropy_train", "token_logprobs_train", "topk_distill_train"]
 
 # the global rows' backward in closed form (_global_bwd); False: autograd over _global_torch
 GLOBAL_BWD_CLOSED_FORM = True
@@ -511,6 +511,65 @@ def cos_scores_train(z: torch.Tensor, table: torch.Tensor, t_rnorm: torch.Tensor
 
 def cross_entropy_train(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     return _CrossEntropy.apply(logits, labels.reshape(-1).to(torch.int64).contiguous(), ignore_index)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    """Log probabilities of given entries and the entropy of softmax(logits * inv_temp), one pass over the
+    logits forward (rf_token_logprobs_fwd) and one backward (rf_token_logprobs_bwd, which recomputes the
+    probabilities from the saved row maxima and sums); the gradient in the logits' type."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, inv_temp: float, ignore_index: int):
+        r = ops.token_logprobs(logits, tokens, inv_temp=inv_temp, ignore_index=ignore_index, want_entropy=True,
+                               want_stats=True)
+        ctx.save_for_backward(logits, tokens, r.stats, r.entropy)
+        ctx.args = (inv_temp, ignore_index)
+        ctx.set_materialize_grads(False)
+        return r.logp, r.entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy):
+        if not ctx.needs_input_grad[0] or (g_logp is None and g_entropy is None):
+            return None, None, None, None
+        logits, tokens, stats, entropy = ctx.saved_tensors
+        inv_temp, ign = ctx.args
+        return ops.token_logprobs_bwd(logits, stats, tokens, g_logp, entropy, g_entropy, inv_temp, ign), None, None, None
+
+
+class _TopkDistill(torch.autograd.Function):
+    """temp^2 times the mean KL of the teacher's best entries from the student's softmax (rf_topk_distill_fwd /
+    rf_topk_distill_bwd); nothing flows to the teacher."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_ids, temp: float):
+        _, stats, loss, coef = ops.topk_distill(logits, teacher_logits, teacher_ids, 1.0 / temp, temp * temp)
+        ctx.save_for_backward(logits, teacher_logits, teacher_ids, stats, coef)
+        ctx.temp = temp
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        if not ctx.needs_input_grad[0]:
+            return None, None, None, None
+        logits, tl, ti, stats, coef = ctx.saved_tensors
+        return ops.topk_distill_bwd(logits, stats, tl, ti, g.float(), coef, 1.0 / ctx.temp), None, None, None
+
+
+def token_logprobs_train(logits: torch.Tensor, tokens: torch.Tensor, inv_temp: float = 1.0, ignore_index: int = -100):
+    """Differentiable (logp, entropy) of ops.token_logprobs: logp fp32 in tokens' shape, entropy (M,) fp32."""
+    return _TokenLogprobs.apply(logits, tokens, float(inv_temp), int(ignore_index))
+
+
+def topk_distill_train(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                       temp: float = 1.0) -> torch.Tensor:
+    """Distillation loss (scalar, fp32): temp^2 * mean over the rows that list something of KL(q || p), with
+    q = softmax(teacher_logits / temp) over teacher_ids and p = softmax(logits / temp) over every column
+    (ops.topk_distill). The factor keeps the gradient's size independent of temp."""
+    if not temp > 0:
+        raise ValueError(f"topk_distill_train: temperature {temp} must be positive")
+    return _TopkDistill.apply(logits, teacher_logits.detach(), teacher_ids, float(temp))
 
 
 class _LMHeadTransform(torch.autograd.Function):
