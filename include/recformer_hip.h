@@ -574,6 +574,24 @@ int rf_topk_distill_bwd(int dtype, int M, int N, const void* logits, int64_t ldx
                         const float* teacher, const int64_t* ids, int K, const float* g, const float* coef,
                         void* dlogits, int64_t ldd, rf_stream_t stream);
 
+/* Microscaled 4-bit floating point (OCP MX, MXFP4): blocks of 32 values along K, a block one scale byte s
+ * (E8M0: 2^(s - 127), 255 = NaN) and 32 E2M1 codes. codes: (M, KB * 16) bytes, 16-byte aligned, the even
+ * element in the low half of its byte; scales: (M, KB) bytes; KB = ceil(K / 32), both contiguous; values past K
+ * are 0. Quantise x (M, K), row stride ldx elements: s = clamp(floor(log2 max|x|) + 125, 0, 254), codes to the
+ * nearest (ties to even, above 6 to 6); a block with inf or NaN: 255. rnorm: (M) fp32 or NULL, 1 / max(|row|,
+ * eps) of the rows before quantisation. */
+int rf_mxfp4_quantize(int dtype, int M, int K, const void* x, int64_t ldx, float eps, uint8_t* codes, uint8_t* scales,
+                      float* rnorm, rf_stream_t stream);
+/* The values codes and scales stand for, rounded to `dtype`: out (M, K), row stride ldo. */
+int rf_mxfp4_dequantize(int dtype, int M, int K, const uint8_t* codes, const uint8_t* scales, void* out, int64_t ldo,
+                        rf_stream_t stream);
+/* C = A . W^T of two such matrices (M rows and N rows of K), fp32 accumulation, then * ra[m] * col_scale * rw[n]
+ * (ra (M) and rw (N) fp32, both or neither: cosine scores) and + bias[n] (fp32 or NULL), rounded once to
+ * out_dtype. C: (M, N), row stride ldc, both it and C's address multiples of four elements. */
+int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* a_codes, const uint8_t* a_scales,
+                  const uint8_t* w_codes, const uint8_t* w_scales, const float* bias, const float* ra, const float* rw,
+                  float col_scale, void* C, int64_t ldc, rf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

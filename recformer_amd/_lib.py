@@ -135,6 +135,9 @@ SIGNATURES = {
                                     P, P]),
     "rf_topk_distill_bwd": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, c_float, P, P, P, c_int, P, P, P,
                                     ctypes.c_int64, P]),
+    "rf_mxfp4_quantize": (c_int, [c_int, c_int, c_int, P, ctypes.c_int64, c_float, P, P, P, P]),
+    "rf_mxfp4_dequantize": (c_int, [c_int, c_int, c_int, P, P, P, ctypes.c_int64, P]),
+    "rf_mxfp4_gemm": (c_int, [c_int, c_int, c_int, c_int, P, P, P, P, P, P, P, c_float, P, ctypes.c_int64, P]),
 }
 
 _LIB: Optional[ctypes.CDLL] = None

@@ -24,6 +24,7 @@ __all__ = [
     "cross_entropy",
     "cos_scores_bwd",
     "TokenLogprobs", "token_logprobs", "token_logprobs_bwd", "topk_distill", "topk_distill_bwd",
+    "Mxfp4", "mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm",
     "RF_EPI_NONE", "RF_EPI_BIAS", "RF_EPI_BIAS_GELU", "RF_EPI_BIAS_GELU_AUX", "RF_EPI_BIAS_RESID", "RF_EPI_COS",
     "RF_EPI_DGELU",
 ]
@@ -1147,4 +1148,94 @@ def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: 
     out, ldd = _like_rows(logits, ld)
     _run(lib.rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
          float(inv_temp), _p(stats), _p(val), _p(ids), ids.shape[1], _p(g), _p(coef), _p(out), ldd)
+    return out
+
+
+# ---- microscaled 4-bit floating point (rf_mxfp4.hip) ------------------------------------------------
+class Mxfp4(NamedTuple):
+    """Rows in MXFP4: codes (M, ceil(k / 32) * 16) uint8 (two E2M1 codes a byte, the even element in the low
+    half), scales (M, ceil(k / 32)) uint8 (E8M0: 2^(s - 127), 255 = NaN), k values a row; contiguous, as
+    mxfp4_quantize writes them. Values past k are 0."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    k: int
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+
+def _mxfp4_check(what: str, q: Mxfp4) -> None:
+    _dev(q.codes, q.scales)
+    kb = (q.k + 31) // 32
+    for t, name, w in ((q.codes, "codes", kb * 16), (q.scales, "scales", kb)):
+        if t.dtype != torch.uint8 or t.dim() != 2 or tuple(t.shape) != (q.codes.shape[0], w) or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} for k={q.k}: contiguous uint8 (rows, {w})")
+    if q.k < 1 or q.codes.data_ptr() % 16 or q.scales.device != q.codes.device:
+        raise ValueError(f"{what}: k must be positive, codes 16-byte aligned, scales beside them")
+
+
+def _mxfp4_rows(x: torch.Tensor, want_rnorm: bool, eps: float):
+    lib = _lib.load()
+    _dev(x)
+    code = dtype_code(x.dtype)
+    ld = _rowmajor(x, "x")
+    M, K = x.shape
+    if K < 1 or (M > 1 and ld < K):
+        raise ValueError(f"mxfp4_quantize: rows of shape {tuple(x.shape)}, strides {x.stride()}")
+    kb = (K + 31) // 32
+    codes = torch.empty(M, kb * 16, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(M, kb, dtype=torch.uint8, device=x.device)
+    rnorm = torch.empty(M, dtype=torch.float32, device=x.device) if want_rnorm else None
+    _run(lib.rf_mxfp4_quantize, "rf_mxfp4_quantize", x, code, M, K, _p(x), max(ld, K), float(eps), _p(codes),
+         _p(scales), _p(rnorm))
+    return Mxfp4(codes, scales, K), rnorm
+
+
+def mxfp4_quantize(x: torch.Tensor, want_rnorm: bool = False, eps: float = 1e-8):
+    """rf_mxfp4_quantize: the rows of a (M, K) bf16 / fp16 / fp32 view in MXFP4 (blocks of 32 along K, scale
+    2^(floor(log2 max) - 2), codes to the nearest, ties to even, above 6 to 6; a block with inf or NaN stands
+    for NaN). want_rnorm: (Mxfp4, 1 / max(row norm, eps)) with the norms of the rows as given, in fp32."""
+    q, rnorm = _mxfp4_rows(x, want_rnorm, eps)
+    return (q, rnorm) if want_rnorm else q
+
+
+def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """rf_mxfp4_dequantize: the (M, k) values q stands for (exact in fp32 and, within its range, bf16)."""
+    lib = _lib.load()
+    _mxfp4_check("mxfp4_dequantize", q)
+    out = torch.empty(q.rows, q.k, dtype=dtype, device=q.codes.device)
+    _run(lib.rf_mxfp4_dequantize, "rf_mxfp4_dequantize", out, dtype_code(dtype), q.rows, q.k, _p(q.codes),
+         _p(q.scales), _p(out), q.k)
+    return out
+
+
+def mxfp4_gemm(a, w: Mxfp4, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               ra: Optional[torch.Tensor] = None, rw: Optional[torch.Tensor] = None, col_scale: float = 1.0,
+               tag: Optional[str] = None) -> torch.Tensor:
+    """rf_mxfp4_gemm: C = a . w^T on the 4-bit matrix cores, fp32 sums, * ra[m] col_scale * rw[n] (cosine scores,
+    as gemm's RF_EPI_COS) and + bias[n], rounded once to out_dtype (default: a's type, fp32 for an Mxfp4). a:
+    (M, K) rows, quantised on the way, or an Mxfp4. The (M, N) result's rows are padded to 16 bytes."""
+    lib = _lib.load()
+    if not isinstance(a, Mxfp4):
+        out_dtype = out_dtype or a.dtype
+        a = mxfp4_quantize(a)
+    out_dtype = out_dtype or torch.float32
+    for q, name in ((a, "a"), (w, "w")):
+        _mxfp4_check(f"mxfp4_gemm: {name}", q)
+    if a.k != w.k:
+        raise ValueError(f"mxfp4_gemm: K mismatch {a.k} vs {w.k}")
+    M, N = a.rows, w.rows
+    dev = a.codes.device
+    if (ra is None) != (rw is None):
+        raise ValueError("mxfp4_gemm: ra and rw go together")
+    for t, n, name in ((bias, N, "bias"), (ra, M, "ra"), (rw, N, "rw"), (w.codes, None, "w")):
+        if t is not None and (t.device != dev or n is not None and
+                              (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous())):
+            raise ValueError(f"mxfp4_gemm: {name} must be contiguous fp32 ({n},) on {dev}")
+    out = torch.empty(M, (N + 7) // 8 * 8, dtype=out_dtype, device=dev)[:, :N]
+    with _region(tag):
+        _run(lib.rf_mxfp4_gemm, "rf_mxfp4_gemm", out, dtype_code(out_dtype), M, N, a.k, _p(a.codes), _p(a.scales),
+             _p(w.codes), _p(w.scales), _p(bias), _p(ra), _p(rw), float(col_scale), _p(out), (N + 7) // 8 * 8)
     return out

@@ -135,6 +135,32 @@ class CatalogShard:
         return self.items.shape[0]
 
 
+class Mxfp4Catalog:
+    """An item table in 4 bits (ops.Mxfp4: 4.25 bits a value) for full-score requests: table, and the inverse
+    norms of the items before quantisation, so that scores() estimates the cosines of the items themselves."""
+
+    def __init__(self, table: ops.Mxfp4, rnorm: torch.Tensor):
+        if rnorm.dtype != torch.float32 or tuple(rnorm.shape) != (table.rows,) or not rnorm.is_contiguous():
+            raise ValueError(f"Mxfp4Catalog: rnorm must be contiguous fp32 ({table.rows},)")
+        self.table = table
+        self.rnorm = rnorm
+
+    @classmethod
+    def from_items(cls, items: torch.Tensor) -> "Mxfp4Catalog":
+        """The catalog of a (N, d) bf16 / fp16 / fp32 item table (Similarity's norm clamp, models.py:366)."""
+        return cls(*ops.mxfp4_quantize(items, want_rnorm=True))
+
+    @property
+    def n(self) -> int:
+        return self.table.rows
+
+    def scores(self, queries: torch.Tensor, temp: float) -> torch.Tensor:
+        """(B, N) fp32 cos(q_b, item_n) / temp (Similarity, models.py:358-369) with queries and items in 4
+        bits; queries (B, d) bf16 / fp16 / fp32, quantised on the way."""
+        q, qn = ops.mxfp4_quantize(queries, want_rnorm=True)
+        return ops.mxfp4_gemm(q, self.table, out_dtype=torch.float32, ra=qn, rw=self.rnorm, col_scale=1.0 / temp)
+
+
 def _check_q(queries: torch.Tensor, shard: CatalogShard) -> torch.Tensor:
     q = queries.contiguous()
     if q.dtype != shard.items.dtype or q.shape[1] != shard.items.shape[1]:
