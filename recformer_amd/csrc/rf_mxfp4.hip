@@ -15,6 +15,7 @@
 #include "rf_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rf {
 
@@ -132,32 +133,41 @@ struct MxArgs {
   float col_scale;
   void* c;
   int64_t ldc;
-  int nTm, nTn, gm;
+  int nTm, nTn, gm, gn;
+  bool vec;  // rows of C are 16-byte aligned
 };
 
-// a and b: fp4 (format 4) in the lower 16 bytes; the scales' byte is picked by an immediate
-template <int OA, int OB>
+// a and b: fp4 (format 4) in the lower 16 bytes, the scales in the lowest byte
 __device__ __forceinline__ f32x4 mfma_mx(u32x4 a, u32x4 b, f32x4 c, uint32_t sa, uint32_t sb) {
   const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
   const i32x8 y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, OA, (int)sa, OB, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
-// four consecutive columns [n, n + 4) of row m
+// what the epilogue takes for four consecutive columns [n, n + 4)
+struct Cols {
+  f32x4 rw, bias;
+};
+template <bool EDGE>
+__device__ __forceinline__ f32x4 load_cols(const float* __restrict__ p, int64_t n, int64_t N, float none) {
+  if (!p) return f32x4{none, none, none, none};
+  if (!EDGE || n + 4 <= N) return *reinterpret_cast<const f32x4*>(p + n);
+  f32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = p[min(n + i, N - 1)];
+  return v;
+}
+__device__ __forceinline__ Cols cols_of(const MxArgs& a, int64_t n) {
+  return {load_cols<true>(a.rw, n, a.N, 1.f), load_cols<true>(a.bias, n, a.N, 0.f)};
+}
+
+// four consecutive columns of row m: (v * ra * rw) + bias, rounded once (without ra: ra = rw = 1, exact)
 template <typename T>
-__device__ __forceinline__ void store4(const MxArgs& a, int64_t m, int64_t n, f32x4 v, float ra) {
-  if (a.ra) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= ra * a.rw[min(n + i, a.N - 1)];
-  }
-  if (a.bias) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += a.bias[min(n + i, a.N - 1)];
-  }
+__device__ __forceinline__ void store4(const MxArgs& a, int64_t m, int64_t n, f32x4 v, float ra, const Cols& c) {
   T* o = (T*)a.c + m * a.ldc + n;
   T e[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(v[i]);
+  for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(fmaf(v[i] * ra, c.rw[i], c.bias[i]));
   if (n + 4 <= a.N) {
     __builtin_memcpy(__builtin_assume_aligned(o, 4 * sizeof(T)), e, sizeof(e));
   } else {
@@ -167,101 +177,285 @@ __device__ __forceinline__ void store4(const MxArgs& a, int64_t m, int64_t n, f3
   }
 }
 
-// 128 x 128 tiles, four waves of 64 x 64, K in steps of 128 (four blocks a row) through two LDS stages.
-// W is the matrix instruction's first operand, so that a lane's four results are neighbours in a row of C.
-// Rows of a stage are 64 bytes; their 16-byte slots are permuted by (row / 4) % 4, so that the 16 rows a
-// fragment read touches at once fall into different banks.
-constexpr int MX_T = 128;
-constexpr int MX_STAGE = 2 * MX_T * 64;  // bytes: W rows, then A rows
-
+__device__ __forceinline__ void put_one(float v, __amdgpu_buffer_rsrc_t rc, int o) {
+  __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rc, o, 0, 0);
+}
 template <typename T>
-__global__ void __launch_bounds__(256, 4) k_mxfp4_gemm(MxArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t code[2][MX_STAGE];
-  __shared__ __attribute__((aligned(16))) uint8_t scl[2][2 * MX_T * 4];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int r = lane & 15, g = lane >> 4;
-  // columns of tiles in groups of gm row tiles: the group's A rows stay in an XCD's L2 while W streams by
-  const int v = xcd_remap(blockIdx.x, gridDim.x);
-  const int grp = v / (a.gm * a.nTn), in = v - grp * a.gm * a.nTn;
-  const int gm = min(a.gm, a.nTm - grp * a.gm);
-  const int64_t m0 = (int64_t)(grp * a.gm + in % gm) * MX_T, n0 = (int64_t)(in / gm) * MX_T;
-  const int KB = a.KB, nk = (KB + 3) >> 2;
-  // staging: a wave instruction fills 16 rows; lane l writes slot l % 4 of row l / 4
-  const int srow = lane >> 2, sch = (lane & 3) ^ ((srow >> 2) & 3);
-  const uint8_t* src[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = (wave * 4 + i) * 16 + srow;  // 0..127: W rows, 128..255: A rows
-    src[i] = row < MX_T ? a.wc + min(n0 + row, a.N - 1) * KB * 16 : a.ac + min(m0 + row - MX_T, a.M - 1) * KB * 16;
-  }
-  const uint8_t* ssrc = t < MX_T ? a.ws + min(n0 + t, a.N - 1) * KB : a.as + min(m0 + t - MX_T, a.M - 1) * KB;
-  const bool sdw = (KB & 3) == 0 && ((reinterpret_cast<uintptr_t>(a.ws) | reinterpret_cast<uintptr_t>(a.as)) & 3) == 0;
-  auto stage = [&](int kt, int b) {
-    const int ch = min(4 * kt + sch, KB - 1);  // past the last block: a block of the row, multiplied by 0 below
-#pragma unroll
-    for (int i = 0; i < 4; ++i) glds16(src[i] + ch * 16, &code[b][(wave * 4 + i) * 1024]);
-  };
-  auto load_scales = [&](int kt) -> uint32_t {
-    if (sdw) return *reinterpret_cast<const uint32_t*>(ssrc + 4 * kt);
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w |= (uint32_t)(4 * kt + i < KB ? ssrc[4 * kt + i] : 127) << (8 * i);
-    return w;
-  };
-  // scales in LDS as the fragments read them: for 64 rows (four 16-row tiles j), byte j of word [block][row % 16]
-  auto put_scales = [&](int b, uint32_t w) {
-    uint8_t* d = &scl[b][(t >> 6) * 256 + (t & 15) * 4 + ((t >> 4) & 3)];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) d[i * 64] = (uint8_t)(w >> (8 * i));
-  };
-  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  stage(0, 0);
-  put_scales(0, load_scales(0));
-  for (int kt = 0; kt < nk; ++kt) {
-    const int b = kt & 1;
-    wait_vmcnt0();
-    __syncthreads();  // stage kt is in LDS; everyone is done with stage kt - 1
-    u32x4 fw[4], fa[4];
+__device__ __forceinline__ void put_one(T v, __amdgpu_buffer_rsrc_t rc, int o) {
+  __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), rc, o, 0, 0);
+}
+
+// up to 64 floats from p[at] on; past p[n - 1] reads as 0
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_of(const float* p, int64_t at, int64_t n) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(p + at), (short)0, (int)max(min(n - at, (int64_t)64), (int64_t)0) * 4,
+                                           0x00020000);
+}
+
+// row and column factors of a wave's 64 x 64 results, loaded before they are needed
+template <typename T>
+struct MxVec {
+  static constexpr int NV = 16 / sizeof(T);  // neighbours a lane holds: 16 bytes
+  static constexpr int NQ = 16 / NV;         // such pieces, 64 bytes apart: piece q holds columns q 4 NV + NV g
+  float ra[4];
+  f32x4 rw[4], bias[4];  // [q (NV / 4) + h]
+  __device__ __forceinline__ void load(const MxArgs& a, int64_t mw, int64_t nw, int r, int g) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int rw = wn + i * 16 + r, rm = MX_T + wm + i * 16 + r, slot = (g ^ ((r >> 2) & 3)) * 16;
-      fw[i] = *reinterpret_cast<const u32x4*>(&code[b][rw * 64 + slot]);
-      fa[i] = *reinterpret_cast<const u32x4*>(&code[b][rm * 64 + slot]);
+      ra[i] = 1.f;
+      rw[i] = f32x4{1.f, 1.f, 1.f, 1.f};
+      bias[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const uint32_t sw = *reinterpret_cast<const uint32_t*>(&scl[b][(wn >> 6) * 256 + (g * 16 + r) * 4]);
-    const uint32_t sa = *reinterpret_cast<const uint32_t*>(&scl[b][(2 + (wm >> 6)) * 256 + (g * 16 + r) * 4]);
-    uint32_t next = 0;
-    if (kt + 1 < nk) {
-      stage(kt + 1, b ^ 1);
-      next = load_scales(kt + 1);
-    }
-    if (4 * kt + g >= KB) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fa[i] = u32x4{0, 0, 0, 0};
-    }
-#define MX_COL(i, j) acc[i][j] = mfma_mx<i, j>(fw[i], fa[j], acc[i][j], sw, sa)
-#define MX_ROW(i) MX_COL(i, 0); MX_COL(i, 1); MX_COL(i, 2); MX_COL(i, 3)
-    MX_ROW(0); MX_ROW(1); MX_ROW(2); MX_ROW(3);
-#undef MX_ROW
-#undef MX_COL
-    if (kt + 1 < nk) put_scales(b ^ 1, next);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t m = m0 + wm + j * 16 + r;
-    if (m < a.M) {
-      const float ra = a.ra ? a.ra[m] * a.col_scale : 1.f;
+    if (a.ra) {
+      const __amdgpu_buffer_rsrc_t rr = part_of(a.ra, mw, a.M), rc = part_of(a.rw, nw, a.N);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t n = n0 + wn + i * 16 + 4 * g;
-        if (n < a.N) store4<T>(a, m, n, acc[i][j], ra);
+        ra[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rr, r * 4 + i * 64, 0, 0));
+        rw[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, col(g, i) * 4, 0, 0));
       }
     }
+    if (a.bias) {
+      const __amdgpu_buffer_rsrc_t rc = part_of(a.bias, nw, a.N);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        bias[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, col(g, i) * 4, 0, 0));
+    }
+  }
+  static __device__ __forceinline__ int col(int g, int i) { return (i / (NV / 4)) * 4 * NV + NV * g + 4 * (i % (NV / 4)); }
+};
+
+// A wave's 64 x 64 results to rows mw.., columns nw..: acc[i][j] holds columns MxMap::wrow(i, 4 g ..) of row
+// j 16 + r. A lane holds 16 bytes of a row at a time, and the same 64 bytes further on: lanes of rows r and r + 1
+// (r even) trade, so that the even lane holds the first piece of both rows and the odd lane the second, and a
+// store writes whole 128-byte lines (64-byte halves took 893 instead of 779 us at 4096 x 125000 fp32).
+// EDGE: element by element, those outside of C at an offset that the buffer store drops.
+template <typename T, bool EDGE>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, int64_t mw, int64_t nw, int r, int g,
+                                            const f32x4 (&acc)[4][4], const MxVec<T>& vec) {
+  constexpr int NV = MxVec<T>::NV, NQ = MxVec<T>::NQ;
+  const bool odd = r & 1;
+  const float scale = a.ra ? a.col_scale : 1.f;
+  const int row = (int)a.ldc * (int)sizeof(T);
+  const int at = (r & ~1) * row + (NV * g + (odd ? 4 * NV : 0)) * (int)sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
+        (T*)a.c + (mw + j * 16) * a.ldc + nw, (short)0, 0x7FFFFFFF, 0x00020000);
+    const float ra = vec.ra[j] * scale;
+#pragma unroll
+    for (int q = 0; q < NQ; q += 2) {
+      u32x4 w[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        T e[NV];
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+          const int i = (q + p) * (NV / 4) + x / 4;
+          e[x] = from_f32<T>(fmaf(acc[i][j][x & 3] * ra, vec.rw[i][x & 3], vec.bias[i][x & 3]));
+        }
+        __builtin_memcpy(&w[p], e, 16);
+      }
+      u32x4 even_row, odd_row;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t n0 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[0][x], 0xB1, 0xF, 0xF, true);
+        const uint32_t n1 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w[1][x], 0xB1, 0xF, 0xF, true);
+        even_row[x] = odd ? n1 : w[0][x];
+        odd_row[x] = odd ? w[1][x] : n0;
+      }
+      if (!EDGE) {  // non-temporal: read by nobody soon, and the tables stay in L2
+        __builtin_amdgcn_raw_buffer_store_b128(even_row, rc, at + q * 64, 0, 2);
+        __builtin_amdgcn_raw_buffer_store_b128(odd_row, rc, at + row + q * 64, 0, 2);
+      } else {
+        const int64_t m = mw + j * 16 + (r & ~1), n = nw + NV * g + (q + (odd ? 1 : 0)) * (4 * NV);
+        T e0[NV], e1[NV];
+        __builtin_memcpy(e0, &even_row, 16);
+        __builtin_memcpy(e1, &odd_row, 16);
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+          const int o = at + q * 64 + x * (int)sizeof(T);
+          put_one(e0[x], rc, m < a.M && n + x < a.N ? o : -4);
+          put_one(e1[x], rc, m + 1 < a.M && n + x < a.N ? o + row : -4);
+        }
+      }
+    }
+  }
+}
+
+// 128 x 128 tiles, four waves of 64 x 64. K goes in steps of 256 (eight blocks, a 128-byte line of a row)
+// through two LDS stages filled by LDS-DMA: while one is multiplied, the next is on its way, across the end
+// of a tile too (a workgroup takes tile after tile, so the next tile's first stage loads during the
+// epilogue); two workgroups a CU. W is the matrix instruction's first operand, so that a lane's results are
+// neighbours in a row of C; with 16-bit results the W rows of a pair of instructions are interleaved by fours,
+// so that a lane holds eight neighbours.
+// Rows of a stage are 128 bytes; their 16-byte slots are permuted by three bits of the row, so that eight
+// neighbouring lanes of a fragment read cover all banks.
+constexpr int MX_T = 128;
+constexpr int MX_CODES = 2 * MX_T * 128;   // bytes of a stage: W rows, then A rows
+constexpr int MX_STAGE = MX_CODES + 2 * MX_T * 8;  // their scales: [word of four][64 rows: x 4 + i]
+constexpr int MX_WGS = 2 * 256;            // workgroups that fit the card
+
+template <typename T>
+struct MxMap {
+  static constexpr bool H = sizeof(T) == 2;
+  // row of the wave's 64 that instruction i's row x stands for, and the permutation of a row's slots
+  static __device__ __forceinline__ int wrow(int i, int x) {
+    return H ? (i >> 1) * 32 + (x >> 2) * 8 + (i & 1) * 4 + (x & 3) : i * 16 + x;
+  }
+  static __device__ __forceinline__ int wkey(int row) { return H ? (row & 3) | ((row >> 3) & 1) << 2 : row & 7; }
+  static __device__ __forceinline__ int akey(int row) { return row & 7; }
+};
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// blocks of gm x gn tiles, columns first within: the block's A and W rows stay in an XCD's L2, and
+// neighbouring pieces of C's rows are written at about the same time
+__device__ __forceinline__ void tile_of(const MxArgs& a, int v, int64_t& m0, int64_t& n0) {
+  v = xcd_remap(v, a.nTm * a.nTn);
+  const int band = v / (a.gm * a.nTn), inb = v - band * a.gm * a.nTn;
+  const int gm = min(a.gm, a.nTm - band * a.gm);
+  const int cg = inb / (gm * a.gn), inc = inb - cg * gm * a.gn;
+  const int gn = min(a.gn, a.nTn - cg * a.gn);
+  m0 = (int64_t)(band * a.gm + inc / gn) * MX_T;
+  n0 = (int64_t)(cg * a.gn + inc % gn) * MX_T;
+}
+
+// DW: KB is a multiple of 4 and the scales are 4-byte aligned, so a row's scales come by LDS-DMA in words
+template <typename T, bool DW>
+__global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
+  typedef MxMap<T> Map;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // (with a static array hipcc would drain every
+                                                                  //  LDS-DMA in flight before an LDS read)
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int KB = a.KB, nk = (KB + 7) >> 3, tiles = a.nTm * a.nTn;
+  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
+  // staging: waves 0 and 1 take the W rows, 2 and 3 the A rows; an instruction fills 8 rows, lane l writes slot
+  // l % 8 of row l / 8. The buffers end with the matrices: what lies behind reads as 0.
+  const bool isw = wave < 2;
+  int vo[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = (wave & 1) * 64 + i * 8 + (lane >> 3);
+    vo[i] = row * KB * 16 + ((lane & 7) ^ (isw ? Map::wkey(row) : Map::akey(row))) * 16;
+  }
+  // a lane of the fragments reads the words of its four rows i at once
+  const int srow = (wave & 1) * 64 + (isw ? Map::wrow(lane & 3, lane >> 2) : (lane & 3) * 16 + (lane >> 2));
+  const int so = srow * KB;
+  const uint8_t* sbase = nullptr;
+  int rows = 0;
+  __amdgpu_buffer_rsrc_t rc, rs;
+  auto aim = [&](int64_t m0, int64_t n0) {
+    rows = (int)min((int64_t)MX_T, isw ? a.N - n0 : a.M - m0);
+    sbase = isw ? a.ws + n0 * KB : a.as + m0 * KB;
+    rc = __builtin_amdgcn_make_buffer_rsrc((void*)(isw ? a.wc + n0 * KB * 16 : a.ac + m0 * KB * 16), (short)0,
+                                           rows * KB * 16, 0x00020000);
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)sbase, (short)0, rows * KB, 0x00020000);
+  };
+  uint32_t pend[2];  // !DW: this thread's row's scales of the stage on its way
+  auto stage = [&](int kt, int b) {
+    uint8_t* dst = smem + b * MX_STAGE;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rc, (__attribute__((address_space(3))) void*)(dst + (wave * 8 + i) * 1024), 16, vo[i], kt * 128, 0, 0);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      if (DW) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void*)(dst + MX_CODES + d * 1024 + wave * 256), 4, so,
+            8 * kt + 4 * d, 0, 0);
+      } else {
+        pend[d] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = 8 * kt + 4 * d + i;
+          pend[d] |= (uint32_t)(srow < rows && at < KB ? sbase[so + at] : 127) << (8 * i);
+        }
+      }
+    }
+  };
+  // fragment reads: the permutation does not depend on i, and block 4 h + g is slot (g ^ key) ^ 4 h
+  const int ow = (wn + Map::wrow(0, r)) * 128 + (g ^ Map::wkey(Map::wrow(0, r))) * 16;
+  const int oa = (MX_T + wm + r) * 128 + (g ^ Map::akey(r)) * 16;
+  const int osw = MX_CODES + (wn + r * 4) * 4, osa = MX_CODES + (MX_T + wm + r * 4) * 4;
+  int v = blockIdx.x, b = 0, relax = 0;
+  int64_t m0, n0;
+  tile_of(a, v, m0, n0);
+  aim(m0, n0);
+  stage(0, 0);
+  while (true) {
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int nv = v + (int)gridDim.x;
+    int64_t m1 = m0, n1 = n0;
+    const bool inside = m0 + MX_T <= a.M && n0 + MX_T <= a.N && a.vec;
+    MxVec<T> vec;
+    for (int kt = 0; kt < nk; ++kt) {
+      uint8_t* cur = smem + b * MX_STAGE;
+      if (!DW) {
+        *reinterpret_cast<uint32_t*>(cur + MX_CODES + t * 4) = pend[0];
+        *reinterpret_cast<uint32_t*>(cur + MX_CODES + 1024 + t * 4) = pend[1];
+      }
+      // the previous tile's stores, younger than this stage's loads, may stay in flight
+      if (DW && kt == 0 && relax) wait_vm<sizeof(T) == 4 ? 16 : 8>();
+      else wait_vm<0>();
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      __builtin_amdgcn_s_barrier();        // the stage is in LDS; everyone is done with the other one
+      asm volatile("" ::: "memory");
+      if (kt + 1 < nk) {
+        stage(kt + 1, b ^ 1);
+      } else {
+        vec.load(a, m0 + wm, n0 + wn, r, g);
+        if (nv < tiles) {
+          tile_of(a, nv, m1, n1);
+          aim(m1, n1);
+          stage(0, b ^ 1);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 fw[4], fa[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          fw[i] = *reinterpret_cast<const u32x4*>(cur + (ow ^ h * 64) + Map::wrow(i, 0) * 128);
+          fa[i] = *reinterpret_cast<const u32x4*>(cur + (oa ^ h * 64) + i * 2048);
+        }
+        u32x4 sw = *reinterpret_cast<const u32x4*>(cur + osw + h * 1024);
+        u32x4 sa = *reinterpret_cast<const u32x4*>(cur + osa + h * 1024);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sw[i] >>= 8 * g;
+          sa[i] >>= 8 * g;
+        }
+        if (8 * kt + 4 * h + 4 > KB && 8 * kt + 4 * h + g >= KB) {  // past the last block: 0 * 1
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            fa[i] = u32x4{0, 0, 0, 0};
+            sw[i] = sa[i] = 127;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = mfma_mx(fw[i], fa[j], acc[i][j], sw[i], sa[j]);
+      }
+      b ^= 1;
+    }
+    int er = r, eg = g;
+    asm volatile("" : "+v"(er), "+v"(eg));  // the epilogue's addresses are not kept through the K loop
+    if (inside) mx_epilogue<T, false>(a, m0 + wm, n0 + wn, er, eg, acc, vec);
+    else mx_epilogue<T, true>(a, m0 + wm, n0 + wn, er, eg, acc, vec);
+    relax = inside;
+    if (nv >= tiles) break;
+    v = nv;
+    m0 = m1;
+    n0 = n1;
   }
 }
 
@@ -303,7 +497,7 @@ __global__ void __launch_bounds__(256) k_mxfp4_skinny(MxArgs a) {
           fa = u32x4{0, 0, 0, 0};
           sa = 127;
         }
-        acc[j] = mfma_mx<0, 0>(fw[u], fa, acc[j], sb, sa);
+        acc[j] = mfma_mx(fw[u], fa, acc[j], sb, sa);
       }
     }
   }
@@ -311,7 +505,7 @@ __global__ void __launch_bounds__(256) k_mxfp4_skinny(MxArgs a) {
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
     const int64_t m = (int64_t)j * 16 + r;
-    if (m < a.M && n < a.N) store4<T>(a, m, n, acc[j], a.ra ? a.ra[m] * a.col_scale : 1.f);
+    if (m < a.M && n < a.N) store4<T>(a, m, n, acc[j], a.ra ? a.ra[m] * a.col_scale : 1.f, cols_of(a, n));
   }
 }
 
@@ -330,7 +524,16 @@ static void launch_gemm(const MxArgs& a, hipStream_t st) {
     else if (a.M <= 32) k_mxfp4_skinny<T, 2><<<grid, 256, 0, st>>>(a);
     else k_mxfp4_skinny<T, 4><<<grid, 256, 0, st>>>(a);
   } else {
-    k_mxfp4_gemm<T><<<(unsigned)((int64_t)a.nTm * a.nTn), 256, 0, st>>>(a);
+    const unsigned grid = (unsigned)std::min(a.nTm * a.nTn, MX_WGS);
+    const bool dw = a.KB % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.as) | reinterpret_cast<uintptr_t>(a.ws)) & 3) == 0;
+    constexpr int lds = 2 * MX_STAGE;
+    if (dw) {
+      (void)hipFuncSetAttribute((const void*)k_mxfp4_gemm<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      k_mxfp4_gemm<T, true><<<grid, 256, lds, st>>>(a);
+    } else {
+      (void)hipFuncSetAttribute((const void*)k_mxfp4_gemm<T, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      k_mxfp4_gemm<T, false><<<grid, 256, lds, st>>>(a);
+    }
   }
 }
 
@@ -343,7 +546,7 @@ using namespace rf;
 extern "C" int rf_mxfp4_quantize(int dtype, int M, int K, const void* x, int64_t ldx, float eps, uint8_t* codes,
                                  uint8_t* scales, float* rnorm, rf_stream_t stream) {
   RF_REQUIRE(dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16, "rf_mxfp4_quantize: bad dtype %d", dtype);
-  RF_REQUIRE(M >= 0 && K > 0 && K <= (1 << 30) && ldx >= K, "rf_mxfp4_quantize: bad shape M=%d K=%d", M, K);
+  RF_REQUIRE(M >= 0 && K > 0 && K <= (1 << 24) && ldx >= K, "rf_mxfp4_quantize: bad shape M=%d K=%d", M, K);
   if (M == 0) return RF_OK;
   RF_REQUIRE(x && codes && scales, "rf_mxfp4_quantize: null pointer");
   const int es = dtype == RF_F32 ? 4 : 2;
@@ -366,7 +569,7 @@ extern "C" int rf_mxfp4_quantize(int dtype, int M, int K, const void* x, int64_t
 extern "C" int rf_mxfp4_dequantize(int dtype, int M, int K, const uint8_t* codes, const uint8_t* scales, void* out,
                                    int64_t ldo, rf_stream_t stream) {
   RF_REQUIRE(dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16, "rf_mxfp4_dequantize: bad dtype %d", dtype);
-  RF_REQUIRE(M >= 0 && K > 0 && K <= (1 << 30) && ldo >= K, "rf_mxfp4_dequantize: bad shape M=%d K=%d", M, K);
+  RF_REQUIRE(M >= 0 && K > 0 && K <= (1 << 24) && ldo >= K, "rf_mxfp4_dequantize: bad shape M=%d K=%d", M, K);
   if (M == 0) return RF_OK;
   RF_REQUIRE(out && codes && scales, "rf_mxfp4_dequantize: null pointer");
   const int es = dtype == RF_F32 ? 4 : 2;
@@ -390,7 +593,7 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
                              const float* rw, float col_scale, void* C, int64_t ldc, rf_stream_t stream) {
   RF_REQUIRE(out_dtype == RF_F32 || out_dtype == RF_BF16 || out_dtype == RF_F16, "rf_mxfp4_gemm: bad dtype %d",
              out_dtype);
-  RF_REQUIRE(M >= 0 && N >= 0 && K > 0 && K <= (1 << 30) && ldc >= N, "rf_mxfp4_gemm: bad shape M=%d N=%d K=%d", M, N,
+  RF_REQUIRE(M >= 0 && N >= 0 && K > 0 && K <= (1 << 24) && ldc >= N, "rf_mxfp4_gemm: bad shape M=%d N=%d K=%d", M, N,
              K);
   if (M == 0 || N == 0) return RF_OK;
   RF_REQUIRE(a_codes && a_scales && w_codes && w_scales && C, "rf_mxfp4_gemm: null pointer");
@@ -399,14 +602,21 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
   RF_REQUIRE(aligned16(a_codes) && aligned16(w_codes), "rf_mxfp4_gemm: codes must be 16-byte aligned");
   RF_REQUIRE((reinterpret_cast<uintptr_t>(C) & (4 * es - 1)) == 0 && ldc % 4 == 0,
              "rf_mxfp4_gemm: the result's rows must be aligned to four elements");
+  RF_REQUIRE(ldc * es <= (1 << 26), "rf_mxfp4_gemm: rows of the result over 64 MB");  // 32-bit offsets over 17 rows
+  RF_REQUIRE(aligned16(bias) && aligned16(rw), "rf_mxfp4_gemm: bias and rw must be 16-byte aligned");
   MxArgs a{};
   a.M = M; a.N = N; a.KB = (K + 31) / 32;
   a.ac = a_codes; a.as = a_scales; a.wc = w_codes; a.ws = w_scales;
   a.bias = bias; a.ra = ra; a.rw = rw; a.col_scale = col_scale; a.c = C; a.ldc = ldc;
+  a.vec = aligned16(C) && ldc * es % 16 == 0;
   a.nTm = (M + MX_T - 1) / MX_T;
   a.nTn = (N + MX_T - 1) / MX_T;
   // row tiles whose codes fill half of an XCD's 4 MB of L2
   a.gm = (int)std::max<int64_t>(1, std::min<int64_t>(a.nTm, (2 << 20) / ((int64_t)MX_T * a.KB * 16)));
+#ifndef RF_GN
+#define RF_GN 4
+#endif
+  a.gn = RF_GN;
   RF_REQUIRE((int64_t)a.nTm * a.nTn < 0x7FFFFFFF, "rf_mxfp4_gemm: too many tiles");
   hipStream_t st = as_stream(stream);
   if (out_dtype == RF_F32) launch_gemm<float>(a, st);

@@ -1216,7 +1216,7 @@ def mxfp4_gemm(a, w: Mxfp4, bias: Optional[torch.Tensor] = None, out_dtype: Opti
                tag: Optional[str] = None) -> torch.Tensor:
     """rf_mxfp4_gemm: C = a . w^T on the 4-bit matrix cores, fp32 sums, * ra[m] col_scale * rw[n] (cosine scores,
     as gemm's RF_EPI_COS) and + bias[n], rounded once to out_dtype (default: a's type, fp32 for an Mxfp4). a:
-    (M, K) rows, quantised on the way, or an Mxfp4. The (M, N) result's rows are padded to 16 bytes."""
+    (M, K) rows, quantised on the way, or an Mxfp4. The (M, N) result's rows are padded to 128 bytes."""
     lib = _lib.load()
     if not isinstance(a, Mxfp4):
         out_dtype = out_dtype or a.dtype
@@ -1234,8 +1234,10 @@ def mxfp4_gemm(a, w: Mxfp4, bias: Optional[torch.Tensor] = None, out_dtype: Opti
         if t is not None and (t.device != dev or n is not None and
                               (t.dtype != torch.float32 or tuple(t.shape) != (n,) or not t.is_contiguous())):
             raise ValueError(f"mxfp4_gemm: {name} must be contiguous fp32 ({n},) on {dev}")
-    out = torch.empty(M, (N + 7) // 8 * 8, dtype=out_dtype, device=dev)[:, :N]
+    line = 128 // out_dtype.itemsize  # rows on 128-byte lines: every store of a tile writes whole lines
+    ldc = (N + line - 1) // line * line
+    out = torch.empty(M, ldc, dtype=out_dtype, device=dev)[:, :N]
     with _region(tag):
         _run(lib.rf_mxfp4_gemm, "rf_mxfp4_gemm", out, dtype_code(out_dtype), M, N, a.k, _p(a.codes), _p(a.scales),
-             _p(w.codes), _p(w.scales), _p(bias), _p(ra), _p(rw), float(col_scale), _p(out), (N + 7) // 8 * 8)
+             _p(w.codes), _p(w.scales), _p(bias), _p(ra), _p(rw), float(col_scale), _p(out), ldc)
     return out
