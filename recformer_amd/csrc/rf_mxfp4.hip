@@ -347,33 +347,33 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
   const uint8_t* sbase = nullptr;
   int rows = 0;
   __amdgpu_buffer_rsrc_t rc, rs;
-  auto aim = [&](int64_t m0, int64_t n0) {
-    rows = (int)min((int64_t)MX_T, isw ? a.N - n0 : a.M - m0);
+  auto aim = [&](int64_t m0, int64_t n0, bool any) {
+    rows = any ? (int)min((int64_t)MX_T, isw ? a.N - n0 : a.M - m0) : 0;
     sbase = isw ? a.ws + n0 * KB : a.as + m0 * KB;
     rc = __builtin_amdgcn_make_buffer_rsrc((void*)(isw ? a.wc + n0 * KB * 16 : a.ac + m0 * KB * 16), (short)0,
                                            rows * KB * 16, 0x00020000);
     rs = __builtin_amdgcn_make_buffer_rsrc((void*)sbase, (short)0, rows * KB, 0x00020000);
   };
-  uint32_t pend[2];  // !DW: this thread's row's scales of the stage on its way
-  auto stage = [&](int kt, int b) {
+  // piece p of a stage: eight of codes, two of scales
+  auto piece = [&](int kt, int b, int p) {
     uint8_t* dst = smem + b * MX_STAGE;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
+    if (p < 8)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rc, (__attribute__((address_space(3))) void*)(dst + (wave * 8 + i) * 1024), 16, vo[i], kt * 128, 0, 0);
+          rc, (__attribute__((address_space(3))) void*)(dst + (wave * 8 + p) * 1024), 16, vo[p], kt * 128, 0, 0);
+    else if (DW)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(dst + MX_CODES + (p - 8) * 1024 + wave * 256), 4, so,
+          8 * kt + 4 * (p - 8), 0, 0);
+  };
+  uint32_t pend[2] = {0, 0};  // !DW: this thread's row's scales of the stage on its way
+  auto scale_bytes = [&](int kt) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
-      if (DW) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (__attribute__((address_space(3))) void*)(dst + MX_CODES + d * 1024 + wave * 256), 4, so,
-            8 * kt + 4 * d, 0, 0);
-      } else {
-        pend[d] = 0;
+      pend[d] = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = 8 * kt + 4 * d + i;
-          pend[d] |= (uint32_t)(srow < rows && at < KB ? sbase[so + at] : 127) << (8 * i);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int at = 8 * kt + 4 * d + i;
+        pend[d] |= (uint32_t)(srow < rows && at < KB ? sbase[so + at] : 127) << (8 * i);
       }
     }
   };
@@ -384,8 +384,10 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
   int v = blockIdx.x, b = 0, relax = 0;
   int64_t m0, n0;
   tile_of(a, v, m0, n0);
-  aim(m0, n0);
-  stage(0, 0);
+  aim(m0, n0, true);
+#pragma unroll
+  for (int p = 0; p < 10; ++p) piece(0, 0, p);
+  if (!DW) scale_bytes(0);
   while (true) {
     f32x4 acc[4][4];
 #pragma unroll
@@ -408,42 +410,62 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
       __builtin_amdgcn_s_barrier();        // the stage is in LDS; everyone is done with the other one
       asm volatile("" ::: "memory");
-      if (kt + 1 < nk) {
-        stage(kt + 1, b ^ 1);
-      } else {
+      u32x4 fw[2][4], fa[2][4], sw[2], sa[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          fw[h][i] = *reinterpret_cast<const u32x4*>(cur + (ow ^ h * 64) + Map::wrow(i, 0) * 128);
+          fa[h][i] = *reinterpret_cast<const u32x4*>(cur + (oa ^ h * 64) + i * 2048);
+        }
+        sw[h] = *reinterpret_cast<const u32x4*>(cur + osw + h * 1024);
+        sa[h] = *reinterpret_cast<const u32x4*>(cur + osa + h * 1024);
+      }
+      // the next stage: of this tile, of the next one, or (an empty buffer, zeros) of none
+      int next = kt + 1;
+      if (next == nk) {
+        next = 0;
         vec.load(a, m0 + wm, n0 + wn, r, g);
-        if (nv < tiles) {
-          tile_of(a, nv, m1, n1);
-          aim(m1, n1);
-          stage(0, b ^ 1);
+        if (nv < tiles) tile_of(a, nv, m1, n1);
+        aim(m1, n1, nv < tiles);
+      }
+      if (!DW) scale_bytes(next);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sw[h][i] >>= 8 * g;
+          sa[h][i] >>= 8 * g;
+        }
+      }
+      if (8 * kt + 8 > KB) {  // past the last block: 0 * 1
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool in = 8 * kt + 4 * h + g < KB;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sw[h][i] = in ? sw[h][i] : 127;
+            sa[h][i] = in ? sa[h][i] : 127;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) fa[h][i][x] = in ? fa[h][i][x] : 0;
+          }
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        u32x4 fw[4], fa[4];
+        // issuing a piece takes some sixty cycles: between matrix instructions they pass unnoticed
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          fw[i] = *reinterpret_cast<const u32x4*>(cur + (ow ^ h * 64) + Map::wrow(i, 0) * 128);
-          fa[i] = *reinterpret_cast<const u32x4*>(cur + (oa ^ h * 64) + i * 2048);
-        }
-        u32x4 sw = *reinterpret_cast<const u32x4*>(cur + osw + h * 1024);
-        u32x4 sa = *reinterpret_cast<const u32x4*>(cur + osa + h * 1024);
+          piece(next, b ^ 1, h * 5 + i);
+          if (i == 3) piece(next, b ^ 1, h * 5 + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sw[i] >>= 8 * g;
-          sa[i] >>= 8 * g;
-        }
-        if (8 * kt + 4 * h + 4 > KB && 8 * kt + 4 * h + g >= KB) {  // past the last block: 0 * 1
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            fa[i] = u32x4{0, 0, 0, 0};
-            sw[i] = sa[i] = 127;
-          }
+          for (int j = 0; j < 4; ++j) acc[i][j] = mfma_mx(fw[h][i], fa[h][j], acc[i][j], sw[h][i], sa[h][j]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = mfma_mx(fw[i], fa[j], acc[i][j], sw[i], sa[j]);
+        for (int x = 0; x < 5; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // one load
+          __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);  // three matrix instructions
+        }
       }
       b ^= 1;
     }
@@ -457,6 +479,7 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
     m0 = m1;
     n0 = n1;
   }
+  wait_vm<0>();  // the last stage's (empty) loads land before the LDS is given away
 }
 
 // Up to 16 MT rows of A: W is read once from memory straight into the fragments, a wave per 16 of its rows,
@@ -613,10 +636,7 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
   a.nTn = (N + MX_T - 1) / MX_T;
   // row tiles whose codes fill half of an XCD's 4 MB of L2
   a.gm = (int)std::max<int64_t>(1, std::min<int64_t>(a.nTm, (2 << 20) / ((int64_t)MX_T * a.KB * 16)));
-#ifndef RF_GN
-#define RF_GN 4
-#endif
-  a.gn = RF_GN;
+  a.gn = 4;  // column tiles side by side: 1 to 32 took within 3% of each other
   RF_REQUIRE((int64_t)a.nTm * a.nTn < 0x7FFFFFFF, "rf_mxfp4_gemm: too many tiles");
   hipStream_t st = as_stream(stream);
   if (out_dtype == RF_F32) launch_gemm<float>(a, st);
