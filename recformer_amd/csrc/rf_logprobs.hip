@@ -31,7 +31,6 @@ constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 constexpr float LP_NINF = -__builtin_inff();
 constexpr int LP_R = 8;         // 16-byte chunks of a row per thread
 constexpr int LP_KMAX = 256;    // alternatives
-constexpr int LP_CAP = 2048;    // candidates a selection holds
 constexpr int LP_LIST = 1024;   // given entries / teacher entries per row
 
 // ---- elements of a row -----------------------------------------------------------------------
@@ -58,6 +57,14 @@ template <> struct Row<f16> {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ float chunk_max(const u32x4& r) {  // NaN is passed over
+  float v = Row<T>::at(r, 0);
+#pragma unroll
+  for (int e = 1; e < Row<T>::V; ++e) v = fmaxf(v, Row<T>::at(r, e));
+  return v;
+}
+
 // A row starts `off` elements into its first aligned 16-byte chunk; chunk j holds the columns
 // [j V - off, j V - off + V). Chunks that reach over an end of the row are read element by element.
 template <typename T>
@@ -65,9 +72,9 @@ __device__ __forceinline__ int row_off(const T* x) {
   return (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
 }
 template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T* x, int64_t c0, int N) {
+__device__ __forceinline__ u32x4 load_chunk(const T* x, int c0, int N) {
   constexpr int V = Row<T>::V;
-  if (c0 >= 0 && c0 + V <= N) return *reinterpret_cast<const u32x4*>(x + c0);
+  if (c0 >= 0 && c0 <= N - V) return *reinterpret_cast<const u32x4*>(x + c0);
   T v[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) v[e] = c0 + e >= 0 && c0 + e < N ? x[c0 + e] : from_f32<T>(LP_NINF);
@@ -125,9 +132,11 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float* red) {
 }
 
 // ---- the k best of a workgroup's entries -------------------------------------------------------
+template <int TPB>
 struct SelectLds {
-  uint64_t cand[LP_CAP];
-  uint32_t key[1024];  // the threads' largest keys; the histogram of the exact search
+  static constexpr int CAP = TPB == 1024 ? 2048 : TPB == 256 ? 1024 : 512;  // candidates, at least LP_KMAX
+  uint64_t cand[CAP];
+  __attribute__((aligned(16))) uint32_t key[TPB < 256 ? 256 : TPB];  // the threads' largest keys; the histogram of the exact search
   int count;
   uint32_t tau;
   uint64_t prefix;
@@ -148,55 +157,59 @@ __device__ __forceinline__ uint32_t upper_bits(const uint32_t (&g)[PER], int k) 
   return tau;
 }
 
-// Collects into s.cand the candidates for the k best of the entries that the threads hold, at least
-// min(k, n) of them and among them the k best, and returns how many. src.each(tau, f) calls f(entry) for
-// every entry of the calling thread whose key is >= tau, src.again(f) for all its entries; tmax: the
-// thread's largest value; nan: some value is NaN (the float compares of the short way would miss it).
+// The k best of a workgroup's entries, in three steps with a barrier after each: every thread enters the key
+// of its largest value into s.key (and thread 0 clears s.count); one wave finds s.tau; every thread collects
+// what passes.
 //
-// Short way: the k-th largest of the threads' maxima is a lower bound of the k-th largest entry (k threads
-// hold one at least as large), and few entries lie above it: G groups of threads let about
-// G ln(G / (G - k)) through (52 for k = 50, G = 1024; 56 for G = 256, which takes a quarter of the counting).
-// One wave finds the bound's upper 16 bits by counting with ballots. Only where more than LP_CAP entries
-// pass (many equal values, or the best all in few threads) an exact search over the 64-bit entries by
-// 8-bit digits follows; its threshold lets exactly min(k, n) through.
-template <int TPB, typename Src>
-__device__ __forceinline__ int select_candidates(const Src& src, float tmax, bool nan, int k, int64_t n, SelectLds& s) {
-  const int t = threadIdx.x;
-  __syncthreads();
-  s.key[t] = key_of(tmax);
-  if (t == 0) {
-    s.count = 0;
-    s.tau = 0;
-  }
-  __syncthreads();
-  if (n > LP_CAP && !nan) {
-    if (t < 64) {
-      constexpr int PER = TPB / 64;
-      uint32_t g[PER];
+// The k-th largest of the threads' maxima is a lower bound of the k-th largest entry (k threads hold one at
+// least as large), and few entries lie above it: G groups of threads let about G ln(G / (G - k)) through (56
+// for k = 50 and G = 256, and G = 1024 would take four times the counting to save 4). Its upper 16 bits do. Where
+// fewer than k threads hold entries the bound is 0 and everything passes.
+template <int TPB>
+__device__ __forceinline__ void find_tau(SelectLds<TPB>& s, int lane, int k) {
+  uint32_t tau;
+  if (TPB == 1024 && k <= 64) {  // groups of four threads
+    uint32_t g[4];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) g[i] = s.key[i * 64 + t];
-      uint32_t tau;
-      if (PER == 16 && k <= 64) {  // groups of four threads
-        uint32_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = max(max(g[i], g[i + 4 % PER]), max(g[i + 8 % PER], g[i + 12 % PER]));
-        tau = upper_bits(q, k);
-      } else {
-        tau = upper_bits(g, k);
-      }
-      if (t == 0) s.tau = tau;
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 q = *reinterpret_cast<const u32x4*>(&s.key[(i * 64 + lane) * 4 % (TPB < 256 ? 256 : TPB)]);
+      g[i] = max(max(q[0], q[1]), max(q[2], q[3]));
     }
-    __syncthreads();
+    tau = upper_bits(g, k);
+  } else if (TPB == 1024) {  // of two: 355 pass for k = 256
+    uint32_t g[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = (i * 64 + lane) * 2 % (TPB < 256 ? 256 : TPB);
+      g[i] = max(s.key[at], s.key[at + 1]);
+    }
+    tau = upper_bits(g, k);
+  } else {
+    uint32_t g[TPB / 64];
+#pragma unroll
+    for (int i = 0; i < TPB / 64; ++i) g[i] = s.key[i * 64 + lane];
+    tau = upper_bits(g, k);
   }
+  if (lane == 0) s.tau = tau;
+}
+
+// Collects into s.cand what passes s.tau, at least min(k, n) entries and among them the k best, and returns how
+// many. src.each(tau, f) calls f(entry) for every entry of the calling thread whose key is >= tau,
+// src.again(f) for all its entries; nan: some value is NaN (the float compares of src.each would miss it).
+// Where more than CAP entries pass (many equal values, or the best all in few threads) an exact search over
+// the 64-bit entries by 8-bit digits follows; its threshold lets exactly min(k, n) through.
+template <int TPB, typename Src>
+__device__ __forceinline__ int collect(const Src& src, bool nan, int k, int64_t n, SelectLds<TPB>& s) {
+  const int t = threadIdx.x;
   auto take = [&](uint64_t e) {
     const int at = atomicAdd(&s.count, 1);
-    if (at < LP_CAP) s.cand[at] = e;
+    if (at < SelectLds<TPB>::CAP) s.cand[at] = e;
   };
   if (!nan) {
-    src.each(n > LP_CAP ? s.tau : 0u, take);
+    src.each(s.tau, take);
     __syncthreads();
     const int c = s.count;
-    if (c <= LP_CAP) return c;
+    if (c <= SelectLds<TPB>::CAP) return c;
   }
   // exact: the digits of the k-th largest entry from the top; stops as soon as a digit's whole bin is taken
   const int kk = (int)(n < k ? n : k);
@@ -231,17 +244,21 @@ __device__ __forceinline__ int select_candidates(const Src& src, float tmax, boo
     if (e >= least) take(e);
   });
   __syncthreads();
-  return min(s.count, LP_CAP);
+  return min(s.count, SelectLds<TPB>::CAP);
 }
 
 // f(rank, entry) for the candidates in list order: entries are all different, so an entry's rank is the
 // number of larger ones
 template <int TPB, typename F>
-__device__ __forceinline__ void rank_candidates(const SelectLds& s, int c, int k, F f) {
+__device__ __forceinline__ void rank_candidates(const SelectLds<TPB>& s, int c, int k, F f) {
   for (int i = threadIdx.x; i < c; i += TPB) {
     const uint64_t e = s.cand[i];
-    int r = 0;
-    for (int j = 0; j < c; ++j) r += s.cand[j] > e;
+    int r = 0, j = 0;
+    for (; j + 4 <= c; j += 4) {  // reads of four together: their latencies overlap
+      const uint64_t a0 = s.cand[j], a1 = s.cand[j + 1], a2 = s.cand[j + 2], a3 = s.cand[j + 3];
+      r += (a0 > e) + (a1 > e) + (a2 > e) + (a3 > e);
+    }
+    for (; j < c; ++j) r += s.cand[j] > e;
     if (r < k) f(r, e);
   }
 }
@@ -316,7 +333,7 @@ __device__ __forceinline__ void finish_row(const LpArgs& a, int r, const T* __re
 }
 
 template <int TPB>
-__device__ __forceinline__ void write_top(const LpArgs& a, int r, float m, float s, const SelectLds& sel, int c) {
+__device__ __forceinline__ void write_top(const LpArgs& a, int r, float m, float s, const SelectLds<TPB>& sel, int c) {
   const bool empty = s == 0.f;
   const float ls = empty ? 0.f : __builtin_amdgcn_logf(s) * LP_LN2;
   rank_candidates<TPB>(sel, c, a.k, [&](int rank, uint64_t e) {
@@ -333,29 +350,25 @@ template <typename T, int TPB>
 struct RowSrc {
   const T* x;
   u32x4* raw;
+  float tmax;          // of the thread's chunks
   int j0, jn, off, N;  // the slice's chunks [j0, j0 + jn)
   template <typename F>
   __device__ __forceinline__ void each(uint32_t tau, F f) const {
     constexpr int V = Row<T>::V;
     // keys at or below -inf's: every column; otherwise an ordinary float compare
-    const bool all = tau <= 0x007FFFFFu;
-    const float lim = all ? LP_NINF : value_of(tau);
+    const float lim = tau <= 0x007FFFFFu ? LP_NINF : value_of(tau);
+    if (!(tmax >= lim)) return;
+    int base = (j0 + (int)threadIdx.x) * V - off, have = jn - (int)threadIdx.x;
+    asm volatile("" : "+v"(base), "+v"(have));
 #pragma unroll
     for (int i = 0; i < LP_R; ++i) {
-      const int j = i * TPB + (int)threadIdx.x;
-      if (j < jn) {
-        asm volatile("" : "+v"(raw[i]));
-        float top = Row<T>::at(raw[i], 0);
+      asm volatile("" : "+v"(raw[i]));
+      if (i * TPB < have && chunk_max<T>(raw[i]) >= lim) {
+        const int c0 = base + i * TPB * V;
 #pragma unroll
-        for (int e = 1; e < V; ++e) top = fmaxf(top, Row<T>::at(raw[i], e));
-        if (all || top >= lim) {
-          asm volatile("" : "+v"(raw[i]));
-          const int64_t c0 = (int64_t)(j0 + j) * V - off;
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float v = Row<T>::at(raw[i], e);
-            if ((all || v >= lim) && c0 + e >= 0 && c0 + e < N) f(entry_of(v, (uint32_t)(c0 + e)));
-          }
+        for (int e = 0; e < V; ++e) {
+          const float v = Row<T>::at(raw[i], e);
+          if (v >= lim && c0 + e >= 0 && c0 + e < N) f(entry_of(v, (uint32_t)(c0 + e)));
         }
       }
     }
@@ -373,8 +386,8 @@ struct RowSrc {
 template <typename T, int TPB, bool ENT, bool TOP>
 __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a, const T* __restrict__ logits) {
   constexpr int V = Row<T>::V;
-  __shared__ float red[32];
-  __shared__ SelectLds sel;
+  __shared__ float redm[16], reds[32];
+  __shared__ SelectLds<TPB> sel;
   const int t = threadIdx.x;
   const int r = blockIdx.x / a.S, sl = blockIdx.x % a.S;
   const T* x = logits + (int64_t)r * a.ld;
@@ -385,18 +398,27 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
 #pragma unroll
   for (int i = 0; i < LP_R; ++i) {
     const int j = i * TPB + t;
-    if (j < jn) raw[i] = load_chunk(x, (int64_t)(j0 + j) * V - off, a.N);
+    if (j < jn) raw[i] = load_chunk(x, (j0 + j) * V - off, a.N);
     else raw[i] = u32x4{Row<T>::FILL, Row<T>::FILL, Row<T>::FILL, Row<T>::FILL};
   }
   float tmax = LP_NINF;
 #pragma unroll
-  for (int i = 0; i < LP_R; ++i)
+  for (int i = 0; i < LP_R; ++i) tmax = fmaxf(tmax, chunk_max<T>(raw[i]));
+  const int wave = t >> 6;
+  const float wmax = wave_max(tmax);
+  if ((t & 63) == 0) redm[wave] = wmax;
+  if (TOP) {
+    sel.key[t] = key_of(tmax);
+    if (t == 0) sel.count = 0;
+  }
+  __syncthreads();
+  float m = redm[0];
 #pragma unroll
-    for (int e = 0; e < V; ++e) tmax = fmaxf(tmax, Row<T>::at(raw[i], e));
-  float m = block_max<TPB>(tmax, red);
+  for (int w = 1; w < TPB / 64; ++w) m = fmaxf(m, redm[w]);
   if (m == LP_NINF) m = 0.f;
-  // per element: subtract, scale, v_exp, one add, and for the entropy a clamp (so that 0 * -inf stays 0;
-  // e^t is 0 from 2^-150 on) and an fma
+  if (TOP && wave == TPB / 64 - 1) find_tau<TPB>(sel, t & 63, a.k);
+  // per element: subtract, scale, v_exp, one add, and for the entropy a clamp (so that 0 * -inf stays 0; e^t is 0
+  // from 2^-150 on) and an fma
   // (the empty asm keeps the values packed between the passes: unpacked they would not fit the registers)
   float s = 0.f, h = 0.f;
 #pragma unroll
@@ -412,9 +434,23 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
       }
     }
   }
-  block_sum2<TPB>(s, h, red);
+  s = wave_sum(s);
+  if (ENT) h = wave_sum(h);
+  if ((t & 63) == 0) {
+    reds[wave] = s;
+    if (ENT) reds[16 + wave] = h;
+  }
+  __syncthreads();
+  s = reds[0];
+  h = ENT ? reds[16] : 0.f;
+#pragma unroll
+  for (int w = 1; w < TPB / 64; ++w) {
+    s += reds[w];
+    if (ENT) h += reds[16 + w];
+  }
+  if (!(s < __builtin_inff())) s = __builtin_nanf("");  // NaN or +inf in the row
   if (a.S == 1) {
-    finish_row<TPB>(a, r, x, m, s, h, red);
+    finish_row<TPB>(a, r, x, m, s, h, reds);
   } else if (t == 0) {
     float* p = a.part + (int64_t)blockIdx.x * 4;
     p[0] = s == 0.f ? LP_NINF : m;
@@ -424,8 +460,8 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
   if (TOP) {
     const int64_t first = max((int64_t)j0 * V - off, (int64_t)0);
     const int64_t n = max(min((int64_t)(j0 + jn) * V - off, (int64_t)a.N) - first, (int64_t)0);
-    const RowSrc<T, TPB> src{x, raw, j0, jn, off, a.N};
-    const int c = select_candidates<TPB>(src, tmax, s != s, a.k, n, sel);
+    const RowSrc<T, TPB> src{x, raw, tmax, j0, jn, off, a.N};
+    const int c = collect<TPB>(src, s != s, a.k, n, sel);
     if (a.S == 1) {
       write_top<TPB>(a, r, m, s, sel, c);
     } else {
@@ -455,7 +491,7 @@ struct ListSrc {
 template <typename T, int TPB, bool TOP>
 __global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __restrict__ logits) {
   __shared__ float red[32];
-  __shared__ SelectLds sel;
+  __shared__ SelectLds<TPB> sel;
   const int t = threadIdx.x, r = blockIdx.x;
   const float* part = a.part + (int64_t)r * a.S * 4;
   float m = LP_NINF;
@@ -477,8 +513,12 @@ __global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __rest
     const ListSrc<TPB> src{a.pent + (int64_t)r * a.S * a.k, a.S * a.k};
     uint64_t best = 0;
     src.again([&](uint64_t e) { best = max(best, e); });
-    const float tmax = best ? value_of((uint32_t)(best >> 32)) : LP_NINF;
-    const int c = select_candidates<TPB>(src, tmax, false, a.k, (int64_t)a.S * a.k, sel);
+    sel.key[t] = (uint32_t)(best >> 32);
+    if (t == 0) sel.count = 0;
+    __syncthreads();
+    if (t < 64) find_tau<TPB>(sel, t, a.k);
+    __syncthreads();
+    const int c = collect<TPB>(src, false, a.k, (int64_t)a.S * a.k, sel);
     write_top<TPB>(a, r, m, s, sel, c);
   }
 }
@@ -541,7 +581,7 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
 #pragma unroll
   for (int i = 0; i < LB_R; ++i) {
     const int j = i * LB_TPB + t;
-    if (j < jn) raw[i] = load_chunk(x, (int64_t)(j0 + j) * V - off, a.N);
+    if (j < jn) raw[i] = load_chunk(x, (j0 + j) * V - off, a.N);
   }
   const float m = a.stats[4 * (int64_t)r], rs = a.stats[4 * (int64_t)r + 1];
   const bool empty = rs == 0.f;
@@ -644,10 +684,13 @@ template <typename T, bool ENT, bool TOP>
 static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
   const T* p = (const T*)x;
   const unsigned grid = (unsigned)((int64_t)a.M * a.S);
-  if (a.cps <= 256 * LP_R) k_logprobs<T, 256, ENT, TOP><<<grid, 256, 0, st>>>(a, p);
+  // one wave a row where rows are short and fill the card; 1024 threads where a slice needs them or many
+  // alternatives want many groups
+  if (a.cps <= 64 * LP_R && a.S == 1 && a.M >= 2048 && a.k <= 16) k_logprobs<T, 64, ENT, TOP><<<grid, 64, 0, st>>>(a, p);
+  else if (a.cps <= 256 * LP_R && a.k <= 64) k_logprobs<T, 256, ENT, TOP><<<grid, 256, 0, st>>>(a, p);
   else k_logprobs<T, 1024, ENT, TOP><<<grid, 1024, 0, st>>>(a, p);
   if (a.S > 1) {
-    if (!TOP || a.S * a.k <= 2048) k_logprobs_join<T, 256, TOP><<<a.M, 256, 0, st>>>(a, p);
+    if (!TOP || (a.S * a.k <= 2048 && a.k <= 64)) k_logprobs_join<T, 256, TOP><<<a.M, 256, 0, st>>>(a, p);
     else k_logprobs_join<T, 1024, TOP><<<a.M, 1024, 0, st>>>(a, p);
   }
 }
@@ -728,7 +771,7 @@ extern "C" int rf_token_logprobs_fwd(int dtype, int M, int N, const void* logits
                                      float* entropy, float* top_logp, int64_t* top_ids, float* stats, void* workspace,
                                      rf_stream_t stream) {
   LpArgs a{};
-  a.M = M; a.N = N; a.ld = ldx; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.M = M; a.N = N; a.ld = ldx; a.it = inv_temp; a.c2 = (float)((double)inv_temp * 1.4426950408889634);
   a.ids = tokens; a.nids = C; a.ignore = ignore_index; a.k = k;
   a.logp = logp; a.entropy = entropy; a.top_logp = top_logp; a.top_ids = top_ids; a.stats = stats;
   return lp_forward("rf_token_logprobs_fwd", dtype, a, logits, workspace, as_stream(stream));
@@ -740,7 +783,7 @@ extern "C" int rf_token_logprobs_bwd(int dtype, int M, int N, const void* logits
                                      int64_t ldd, rf_stream_t stream) {
   RF_REQUIRE(!g_entropy || entropy, "rf_token_logprobs_bwd: the entropy's gradient needs the entropy");
   LpBwdArgs a{};
-  a.M = M; a.N = N; a.ld = ldx; a.ldd = ldd; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.M = M; a.N = N; a.ld = ldx; a.ldd = ldd; a.it = inv_temp; a.c2 = (float)((double)inv_temp * 1.4426950408889634);
   a.ids = tokens; a.nids = C; a.ignore = ignore_index; a.g = g_logp; a.entropy = entropy; a.g_ent = g_entropy;
   a.stats = stats;
   return lp_backward("rf_token_logprobs_bwd", dtype, a, logits, dlogits, as_stream(stream));
@@ -753,7 +796,7 @@ extern "C" int rf_topk_distill_fwd(int dtype, int M, int N, const void* logits, 
   RF_REQUIRE(M <= 0 || (teacher && rows && stats), "rf_topk_distill_fwd: null pointer");
   RF_REQUIRE(!loss == !coef, "rf_topk_distill_fwd: loss and coef go together");
   LpArgs a{};
-  a.M = M; a.N = N; a.ld = ldx; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.M = M; a.N = N; a.ld = ldx; a.it = inv_temp; a.c2 = (float)((double)inv_temp * 1.4426950408889634);
   a.ids = ids; a.nids = K; a.tval = teacher; a.logp = rows; a.stats = stats;
   const int rc = lp_forward("rf_topk_distill_fwd", dtype, a, logits, workspace, as_stream(stream));
   if (rc != RF_OK || !loss) return rc;
@@ -767,7 +810,7 @@ extern "C" int rf_topk_distill_bwd(int dtype, int M, int N, const void* logits, 
   RF_REQUIRE(K >= 1, "rf_topk_distill_bwd: K=%d teacher entries", K);
   RF_REQUIRE(M <= 0 || (teacher && g && coef), "rf_topk_distill_bwd: null pointer");
   LpBwdArgs a{};
-  a.M = M; a.N = N; a.ld = ldx; a.ldd = ldd; a.it = inv_temp; a.c2 = inv_temp * LP_LOG2E;
+  a.M = M; a.N = N; a.ld = ldx; a.ldd = ldd; a.it = inv_temp; a.c2 = (float)((double)inv_temp * 1.4426950408889634);
   a.ids = ids; a.nids = K; a.tval = teacher; a.g = g; a.coef = coef; a.stats = stats;
   return lp_backward("rf_topk_distill_bwd", dtype, a, logits, dlogits, as_stream(stream));
 }
