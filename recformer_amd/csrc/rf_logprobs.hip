@@ -39,11 +39,13 @@ template <typename T> struct Row;
 template <> struct Row<float> {
   static constexpr int V = 4;
   static constexpr uint32_t FILL = 0xFF800000u;
+  static constexpr bool ROUND = true;  // its values do not all fit bf16
   static __device__ __forceinline__ float at(const u32x4& r, int e) { return __uint_as_float(r[e]); }
 };
 template <> struct Row<bf16> {
   static constexpr int V = 8;
   static constexpr uint32_t FILL = 0xFF80FF80u;
+  static constexpr bool ROUND = false;
   static __device__ __forceinline__ float at(const u32x4& r, int e) {
     return __uint_as_float(e & 1 ? r[e >> 1] & 0xFFFF0000u : r[e >> 1] << 16);
   }
@@ -51,6 +53,7 @@ template <> struct Row<bf16> {
 template <> struct Row<f16> {
   static constexpr int V = 8;
   static constexpr uint32_t FILL = 0xFC00FC00u;
+  static constexpr bool ROUND = true;
   static __device__ __forceinline__ float at(const u32x4& r, int e) {
     const uint32_t w = r[e >> 1];  // (a bit cast of the vector's element itself would read element 0)
     return (float)__builtin_bit_cast(f16x2, w)[e & 1];
@@ -99,36 +102,44 @@ __device__ __forceinline__ uint64_t entry_of(float v, uint32_t col) {
 }
 
 // ---- workgroup reductions ----------------------------------------------------------------------
+// the waves' results joined by every wave from LDS, a value a lane (read side by side, sixteen values would not
+// fit the registers beside a row)
+template <int TPB>
+__device__ __forceinline__ float waves_max(const float* red) {
+  constexpr int W = TPB / 64;
+  float v = red[threadIdx.x & (W - 1)];
+#pragma unroll
+  for (int o = W >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <int TPB>
+__device__ __forceinline__ float waves_sum(const float* red) {
+  constexpr int W = TPB / 64;
+  float v = red[threadIdx.x & (W - 1)];
+#pragma unroll
+  for (int o = W >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
 template <int TPB>
 __device__ __forceinline__ float block_max(float v, float* red) {
   v = wave_max(v);
-  if (TPB == 64) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int w = 1; w < TPB / 64; ++w) v = fmaxf(v, red[w]);
-  return v;
+  return waves_max<TPB>(red);
 }
 template <int TPB>
 __device__ __forceinline__ void block_sum2(float& a, float& b, float* red) {
   a = wave_sum(a);
   b = wave_sum(b);
-  if (TPB == 64) return;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
     red[threadIdx.x >> 6] = a;
     red[16 + (threadIdx.x >> 6)] = b;
   }
   __syncthreads();
-  a = red[0];
-  b = red[16];
-#pragma unroll
-  for (int w = 1; w < TPB / 64; ++w) {
-    a += red[w];
-    b += red[16 + w];
-  }
+  a = waves_sum<TPB>(red);
+  b = waves_sum<TPB>(red + 16);
 }
 
 // ---- the k best of a workgroup's entries -------------------------------------------------------
@@ -248,7 +259,7 @@ __device__ __forceinline__ int collect(const Src& src, bool nan, int k, int64_t 
 }
 
 // f(rank, entry) for the candidates in list order: entries are all different, so an entry's rank is the
-// number of larger ones
+// number of larger ones (counted by one lane each: several lanes an entry took 4% longer at 4915 x 50265)
 template <int TPB, typename F>
 __device__ __forceinline__ void rank_candidates(const SelectLds<TPB>& s, int c, int k, F f) {
   for (int i = threadIdx.x; i < c; i += TPB) {
@@ -282,45 +293,63 @@ struct LpArgs {
   uint64_t* pent;            // (M S, k) entries, 0 = none
 };
 
+// The thread's entry of a row's list (entry t; the lists' rest is read where it is needed): loaded before the
+// row, its logit after it, so that the row's end does not wait for them.
+template <bool TEACH>
+struct Listed {
+  int32_t id;  // -1: ignored or not used, -2: out of range
+  float t, x;  // teacher logit; logit of the row
+  __device__ __forceinline__ void load(const LpArgs& a, int r, int j) {
+    const int64_t k = j < a.nids ? a.ids[(int64_t)r * a.nids + j] : -1;
+    id = k == (TEACH ? -1 : a.ignore) ? -1 : k >= 0 && k < a.N ? (int32_t)k : -2;
+    if (TEACH) t = j < a.nids ? a.tval[(int64_t)r * a.nids + j] : 0.f;
+  }
+  template <typename T>
+  __device__ __forceinline__ void look(const T* __restrict__ row) {
+    x = id >= 0 ? to_f32(row[id]) : __builtin_nanf("");
+  }
+};
+
 // m, s and h = sum e^t t log2(e) of row r are known to the whole workgroup
-template <int TPB, typename T>
-__device__ __forceinline__ void finish_row(const LpArgs& a, int r, const T* __restrict__ x, float m, float s, float h,
-                                           float* red) {
+template <int TPB, bool TEACH, typename T>
+__device__ __forceinline__ void finish_row(const LpArgs& a, int r, const T* __restrict__ row, float m, float s, float h,
+                                           const Listed<TEACH>& own, float* red) {
   const int t = threadIdx.x;
   const bool empty = s == 0.f;
   const float ls = empty ? 0.f : __builtin_amdgcn_logf(s) * LP_LN2;
-  auto logp_at = [&](int64_t id) {
-    const float v = to_f32(x[id]);
-    return empty || v == LP_NINF ? (s != s ? s : LP_NINF) : (v - m) * a.it - ls;
+  // own.x is NaN for an id out of range
+  auto logp = [&](float v) { return v != v ? v : empty || v == LP_NINF ? (s != s ? s : LP_NINF) : (v - m) * a.it - ls; };
+  auto each = [&](auto f) {
+    if (t < a.nids) f(t, own);
+    for (int j = t + TPB; j < a.nids; j += TPB) {
+      Listed<TEACH> l;
+      l.load(a, r, j);
+      l.look(row);
+      f(j, l);
+    }
   };
   float tm = 0.f, trs = 0.f;
-  if (a.tval) {
-    const int64_t* id = a.ids + (int64_t)r * a.nids;
-    const float* tv = a.tval + (int64_t)r * a.nids;
+  if constexpr (TEACH) {
     float mx = LP_NINF;
-    for (int j = t; j < a.nids; j += TPB)
-      if (id[j] != -1) mx = fmaxf(mx, tv[j]);
+    each([&](int, const Listed<TEACH>& l) {
+      if (l.id != -1) mx = fmaxf(mx, l.t);
+    });
     tm = block_max<TPB>(mx, red);
     if (tm == LP_NINF) tm = 0.f;
     float ts = 0.f, cross = 0.f;
-    for (int j = t; j < a.nids; j += TPB) {
-      if (id[j] == -1) continue;
-      const float tz = (tv[j] - tm) * a.it;
+    each([&](int, const Listed<TEACH>& l) {
+      if (l.id == -1) return;
+      const float tz = (l.t - tm) * a.it;
       const float e = __builtin_amdgcn_exp2f(tz * LP_LOG2E);
       ts += e;
-      // a teacher logit of -inf teaches nothing, whatever the student says
-      if (e != 0.f) cross += e * (tz - (id[j] >= 0 && id[j] < a.N ? logp_at(id[j]) : __builtin_nanf("")));
-    }
+      if (e != 0.f) cross += e * (tz - logp(l.x));  // a teacher logit of -inf teaches nothing, whatever the student says
+    });
     block_sum2<TPB>(ts, cross, red);
     trs = ts == 0.f ? 0.f : 1.f / ts;
     // sum q (tz - ln ts - logp) with q = e / ts
     if (t == 0) a.logp[r] = ts == 0.f ? 0.f : cross * trs - __builtin_amdgcn_logf(ts) * LP_LN2;
   } else {
-    for (int j = t; j < a.nids; j += TPB) {
-      const int64_t id = a.ids[(int64_t)r * a.nids + j];
-      a.logp[(int64_t)r * a.nids + j] =
-          id == a.ignore ? 0.f : id >= 0 && id < a.N ? logp_at(id) : __builtin_nanf("");
-    }
+    each([&](int j, const Listed<TEACH>& l) { a.logp[(int64_t)r * a.nids + j] = l.id == -1 ? 0.f : logp(l.x); });
     if (t == 0 && a.entropy) a.entropy[r] = empty ? 0.f : ls - h / s * LP_LN2;
   }
   if (t == 0 && a.stats) {
@@ -350,20 +379,19 @@ template <typename T, int TPB>
 struct RowSrc {
   const T* x;
   u32x4* raw;
-  float tmax;          // of the thread's chunks
+  const uint32_t* top;  // the chunks' maxima rounded up to bf16
   int j0, jn, off, N;  // the slice's chunks [j0, j0 + jn)
   template <typename F>
   __device__ __forceinline__ void each(uint32_t tau, F f) const {
     constexpr int V = Row<T>::V;
     // keys at or below -inf's: every column; otherwise an ordinary float compare
     const float lim = tau <= 0x007FFFFFu ? LP_NINF : value_of(tau);
-    if (!(tmax >= lim)) return;
     int base = (j0 + (int)threadIdx.x) * V - off, have = jn - (int)threadIdx.x;
     asm volatile("" : "+v"(base), "+v"(have));
 #pragma unroll
     for (int i = 0; i < LP_R; ++i) {
-      asm volatile("" : "+v"(raw[i]));
-      if (i * TPB < have && chunk_max<T>(raw[i]) >= lim) {
+      if (i * TPB < have && __uint_as_float(i & 1 ? top[i / 2] & 0xFFFF0000u : top[i / 2] << 16) >= lim) {
+        asm volatile("" : "+v"(raw[i]));
         const int c0 = base + i * TPB * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -383,7 +411,7 @@ struct RowSrc {
 };
 
 // ---- one slice of a row ------------------------------------------------------------------------
-template <typename T, int TPB, bool ENT, bool TOP>
+template <typename T, int TPB, bool ENT, bool TOP, bool TEACH>
 __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a, const T* __restrict__ logits) {
   constexpr int V = Row<T>::V;
   __shared__ float redm[16], reds[32];
@@ -394,6 +422,8 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
   const int off = row_off(x);
   const int nch = (int)(((int64_t)a.N + off + V - 1) / V);
   const int j0 = min(sl * a.cps, nch), jn = min(a.cps, nch - j0);
+  Listed<TEACH> own;
+  if (a.S == 1) own.load(a, r, t);
   u32x4 raw[LP_R];
 #pragma unroll
   for (int i = 0; i < LP_R; ++i) {
@@ -402,8 +432,17 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
     else raw[i] = u32x4{Row<T>::FILL, Row<T>::FILL, Row<T>::FILL, Row<T>::FILL};
   }
   float tmax = LP_NINF;
+  uint32_t top[LP_R / 2];  // the chunks' maxima rounded up to bf16, two a word
 #pragma unroll
-  for (int i = 0; i < LP_R; ++i) tmax = fmaxf(tmax, chunk_max<T>(raw[i]));
+  for (int i = 0; i < LP_R; ++i) {
+    const float v = chunk_max<T>(raw[i]);
+    tmax = fmaxf(tmax, v);
+    if (TOP) {
+      const uint32_t b = __float_as_uint(v), up = Row<T>::ROUND ? (b >> 31 ? b : b + 0xFFFFu) : b;
+      top[i / 2] = i & 1 ? top[i / 2] | (up & 0xFFFF0000u) : up >> 16;
+    }
+  }
+  if (a.S == 1) own.look(x);
   const int wave = t >> 6;
   const float wmax = wave_max(tmax);
   if ((t & 63) == 0) redm[wave] = wmax;
@@ -412,9 +451,7 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
     if (t == 0) sel.count = 0;
   }
   __syncthreads();
-  float m = redm[0];
-#pragma unroll
-  for (int w = 1; w < TPB / 64; ++w) m = fmaxf(m, redm[w]);
+  float m = waves_max<TPB>(redm);
   if (m == LP_NINF) m = 0.f;
   if (TOP && wave == TPB / 64 - 1) find_tau<TPB>(sel, t & 63, a.k);
   // per element: subtract, scale, v_exp, one add, and for the entropy a clamp (so that 0 * -inf stays 0; e^t is 0
@@ -441,16 +478,11 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
     if (ENT) reds[16 + wave] = h;
   }
   __syncthreads();
-  s = reds[0];
-  h = ENT ? reds[16] : 0.f;
-#pragma unroll
-  for (int w = 1; w < TPB / 64; ++w) {
-    s += reds[w];
-    if (ENT) h += reds[16 + w];
-  }
+  s = waves_sum<TPB>(reds);
+  h = ENT ? waves_sum<TPB>(reds + 16) : 0.f;
   if (!(s < __builtin_inff())) s = __builtin_nanf("");  // NaN or +inf in the row
   if (a.S == 1) {
-    finish_row<TPB>(a, r, x, m, s, h, reds);
+    finish_row<TPB, TEACH>(a, r, x, m, s, h, own, reds);
   } else if (t == 0) {
     float* p = a.part + (int64_t)blockIdx.x * 4;
     p[0] = s == 0.f ? LP_NINF : m;
@@ -460,7 +492,7 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
   if (TOP) {
     const int64_t first = max((int64_t)j0 * V - off, (int64_t)0);
     const int64_t n = max(min((int64_t)(j0 + jn) * V - off, (int64_t)a.N) - first, (int64_t)0);
-    const RowSrc<T, TPB> src{x, raw, tmax, j0, jn, off, a.N};
+    const RowSrc<T, TPB> src{x, raw, top, j0, jn, off, a.N};
     const int c = collect<TPB>(src, s != s, a.k, n, sel);
     if (a.S == 1) {
       write_top<TPB>(a, r, m, s, sel, c);
@@ -488,11 +520,15 @@ struct ListSrc {
   __device__ __forceinline__ void again(F f) const { each(0u, f); }
 };
 
-template <typename T, int TPB, bool TOP>
+template <typename T, int TPB, bool TOP, bool TEACH>
 __global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __restrict__ logits) {
   __shared__ float red[32];
   __shared__ SelectLds<TPB> sel;
   const int t = threadIdx.x, r = blockIdx.x;
+  const T* x = logits + (int64_t)r * a.ld;
+  Listed<TEACH> own;
+  own.load(a, r, t);
+  own.look(x);
   const float* part = a.part + (int64_t)r * a.S * 4;
   float m = LP_NINF;
   for (int i = t; i < a.S; i += TPB) m = fmaxf(m, part[4 * i]);
@@ -508,7 +544,7 @@ __global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __rest
     h = fmaf(f, fmaf(fmaxf(d, -200.f), si, part[4 * i + 2]), h);
   }
   block_sum2<TPB>(s, h, red);
-  finish_row<TPB>(a, r, logits + (int64_t)r * a.ld, m, s, h, red);
+  finish_row<TPB, TEACH>(a, r, x, m, s, h, own, red);
   if (TOP) {
     const ListSrc<TPB> src{a.pent + (int64_t)r * a.S * a.k, a.S * a.k};
     uint64_t best = 0;
@@ -680,18 +716,21 @@ static void lp_plan(int dtype, int M, int N, int k, int* S, int* cps) {
   *S = (int)((nch + *cps - 1) / *cps);
 }
 
-template <typename T, bool ENT, bool TOP>
+template <typename T, bool ENT, bool TOP, bool TEACH>
 static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
   const T* p = (const T*)x;
   const unsigned grid = (unsigned)((int64_t)a.M * a.S);
   // one wave a row where rows are short and fill the card; 1024 threads where a slice needs them or many
   // alternatives want many groups
-  if (a.cps <= 64 * LP_R && a.S == 1 && a.M >= 2048 && a.k <= 16) k_logprobs<T, 64, ENT, TOP><<<grid, 64, 0, st>>>(a, p);
-  else if (a.cps <= 256 * LP_R && a.k <= 64) k_logprobs<T, 256, ENT, TOP><<<grid, 256, 0, st>>>(a, p);
-  else k_logprobs<T, 1024, ENT, TOP><<<grid, 1024, 0, st>>>(a, p);
+  if (a.cps <= 64 * LP_R && a.S == 1 && a.M >= 2048 && a.k <= 16)
+    k_logprobs<T, 64, ENT, TOP, TEACH><<<grid, 64, 0, st>>>(a, p);
+  else if (a.cps <= 256 * LP_R && a.k <= 64)
+    k_logprobs<T, 256, ENT, TOP, TEACH><<<grid, 256, 0, st>>>(a, p);
+  else
+    k_logprobs<T, 1024, ENT, TOP, TEACH><<<grid, 1024, 0, st>>>(a, p);
   if (a.S > 1) {
-    if (!TOP || (a.S * a.k <= 2048 && a.k <= 64)) k_logprobs_join<T, 256, TOP><<<a.M, 256, 0, st>>>(a, p);
-    else k_logprobs_join<T, 1024, TOP><<<a.M, 1024, 0, st>>>(a, p);
+    if (!TOP || (a.S * a.k <= 2048 && a.k <= 64)) k_logprobs_join<T, 256, TOP, TEACH><<<a.M, 256, 0, st>>>(a, p);
+    else k_logprobs_join<T, 1024, TOP, TEACH><<<a.M, 1024, 0, st>>>(a, p);
   }
 }
 
@@ -714,11 +753,12 @@ static int lp_forward(const char* name, int dtype, const LpArgs& in, const void*
     a.pent = (uint64_t*)((char*)ws + (size_t)a.M * a.S * 16);
   }
   const bool ent = a.entropy != nullptr, top = a.k > 0;
-#define LP_T(T)                                                 \
-  if (ent && top) lp_launch<T, true, true>(a, logits, st);      \
-  else if (ent) lp_launch<T, true, false>(a, logits, st);       \
-  else if (top) lp_launch<T, false, true>(a, logits, st);       \
-  else lp_launch<T, false, false>(a, logits, st)
+#define LP_T(T)                                                        \
+  if (a.tval) lp_launch<T, false, false, true>(a, logits, st);         \
+  else if (ent && top) lp_launch<T, true, true, false>(a, logits, st); \
+  else if (ent) lp_launch<T, true, false, false>(a, logits, st);       \
+  else if (top) lp_launch<T, false, true, false>(a, logits, st);       \
+  else lp_launch<T, false, false, false>(a, logits, st)
   if (dtype == RF_F32) { LP_T(float); }
   else if (dtype == RF_BF16) { LP_T(bf16); }
   else { LP_T(f16); }

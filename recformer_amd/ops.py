@@ -990,45 +990,51 @@ class TokenLogprobs(NamedTuple):
 
 def _run(fn, what: str, ref: torch.Tensor, *args) -> None:
     """fn(*args, stream) on ref's device (made current for the call where it is not) and its current stream."""
-    if ref.device.index == torch.cuda.current_device():
-        check(fn(*args, _stream(ref)), what)
+    dev = ref.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(ref.device):
-            check(fn(*args, _stream(ref)), what)
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
 
 
-def _logit_rows(what: str, logits: torch.Tensor, inv_temp: float) -> int:
-    """Checks a (M, N) row-major view and the inverse temperature; its row stride."""
+def _logit_rows(what: str, logits: torch.Tensor, inv_temp: float):
+    """Checks a (M, N) row-major view and the inverse temperature: (type code, M, N, address, row stride,
+    inverse temperature), as the entry points take them."""
     _dev(logits)
-    dtype_code(logits.dtype)
+    code = dtype_code(logits.dtype)
     ld = _rowmajor(logits, "logits")
     M, N = logits.shape
     if N < 1 or N >= 2 ** 31 - 16 or M >= 2 ** 31:
         raise ValueError(f"{what}: logits {tuple(logits.shape)}")
     if M > 1 and ld < N:
         raise ValueError(f"{what}: rows of the logits overlap (stride {ld} < {N})")
-    if not (inv_temp > 0 and math.isfinite(inv_temp)):
+    inv_temp = float(inv_temp)
+    if not 0.0 < inv_temp < math.inf:
         raise ValueError(f"{what}: inverse temperature {inv_temp} must be positive and finite")
-    return max(ld, N)
+    return code, M, N, logits.data_ptr(), max(ld, N), inv_temp
 
 
-def _row_list(what: str, t: torch.Tensor, logits: torch.Tensor, dtype=None) -> torch.Tensor:
-    """A contiguous (M, C) list beside the logits' rows: int64 ids, or values in `dtype`."""
-    if t.device != logits.device:
+def _row_list(what: str, t: torch.Tensor, logits: torch.Tensor, dtype: torch.dtype = torch.int64) -> torch.Tensor:
+    """A contiguous (M, C) list beside the logits' rows: int64 ids, or fp32 values."""
+    if t.get_device() != logits.get_device():
         raise ValueError(f"{what}: on {t.device}, logits on {logits.device}")
-    if dtype is None and t.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"{what}: int64 or int32 ids, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != logits.shape[0] or t.shape[1] > 1024:
         raise ValueError(f"{what}: shape {tuple(t.shape)} for {logits.shape[0]} rows (up to 1024 entries each)")
-    return t.to(dtype or torch.int64).contiguous()
+    if t.dtype != dtype:
+        if dtype == torch.int64 and t.dtype != torch.int32:
+            raise TypeError(f"{what}: int64 or int32 ids, got {t.dtype}")
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _like_rows(logits: torch.Tensor, ld: int) -> Tuple[torch.Tensor, int]:
     """An empty (M, N) tensor whose rows are aligned as the logits' rows are (contiguous where theirs allow it)."""
     M, N = logits.shape
     es = logits.element_size()
-    v = 16 // es
-    ldd = N + (ld - N) % v
+    ldd = N + (ld - N) % (16 // es)
     off = logits.data_ptr() % 16 // es
     if off == 0 and ldd == N:
         return torch.empty(M, N, dtype=logits.dtype, device=logits.device), ldd
@@ -1036,9 +1042,13 @@ def _like_rows(logits: torch.Tensor, ld: int) -> Tuple[torch.Tensor, int]:
     return buf.as_strided((M, N), (ldd, 1), off), ldd
 
 
-def _logprobs_ws(lib, logits: torch.Tensor, k: int) -> Optional[torch.Tensor]:
-    n = lib.rf_logprobs_workspace(dtype_code(logits.dtype), logits.shape[0], logits.shape[1], k)
-    return torch.empty(n, dtype=torch.uint8, device=logits.device) if n else None
+def _logprobs_ws(lib, code: int, M: int, N: int, k: int, dev) -> Optional[torch.Tensor]:
+    n = lib.rf_logprobs_workspace(code, M, N, k)
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _token_ids(what: str, tokens: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+    return _row_list(what, tokens.unsqueeze(1) if tokens.dim() == 1 else tokens, logits)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, k: int = 0, inv_temp: float = 1.0,
@@ -1048,26 +1058,26 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     other id outside [0, N) NaN), the entropy, and the k <= 256 best alternatives (largest logit first, the
     lower id first among equals). Masked columns are -inf; a row of nothing else gives -inf, entropy 0."""
     lib = _lib.load()
-    ld = _logit_rows("token_logprobs", logits, inv_temp)
-    M, N = logits.shape
+    rows = _logit_rows("token_logprobs", logits, inv_temp)
+    code, M, N = rows[:3]
     if not 0 <= k <= min(N, 256):
         raise ValueError(f"token_logprobs: k={k} must be in [0, min(N, 256)]")
+    dev, f32 = logits.device, torch.float32
     ids = logp = None
     C = 0
     if tokens is not None:
-        ids = _row_list("token_logprobs: tokens", tokens.unsqueeze(1) if tokens.dim() == 1 else tokens, logits)
+        ids = _token_ids("token_logprobs: tokens", tokens, logits)
         C = ids.shape[1]
-        logp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+        logp = torch.empty(tokens.shape, dtype=f32, device=dev)
     elif not (k or want_entropy or want_stats):
         raise ValueError("token_logprobs: no output requested")
-    dev = logits.device
-    ent = torch.empty(M, dtype=torch.float32, device=dev) if want_entropy else None
-    tv = torch.empty(M, k, dtype=torch.float32, device=dev) if k else None
+    ent = torch.empty(M, dtype=f32, device=dev) if want_entropy else None
+    tv = torch.empty(M, k, dtype=f32, device=dev) if k else None
     ti = torch.empty(M, k, dtype=torch.int64, device=dev) if k else None
-    stats = torch.empty(M, 4, dtype=torch.float32, device=dev) if want_stats else None
-    ws = _logprobs_ws(lib, logits, k)
-    _run(lib.rf_token_logprobs_fwd, "rf_token_logprobs_fwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
-         float(inv_temp), _p(ids), C, int(ignore_index), k, _p(logp), _p(ent), _p(tv), _p(ti), _p(stats), _p(ws))
+    stats = torch.empty(M, 4, dtype=f32, device=dev) if want_stats else None
+    ws = _logprobs_ws(lib, code, M, N, k, dev)
+    _run(lib.rf_token_logprobs_fwd, "rf_token_logprobs_fwd", logits, *rows, _p(ids), C, int(ignore_index), k, _p(logp),
+         _p(ent), _p(tv), _p(ti), _p(stats), _p(ws))
     return TokenLogprobs(logp, ent, tv, ti, stats)
 
 
@@ -1077,29 +1087,38 @@ def token_logprobs_bwd(logits: torch.Tensor, stats: torch.Tensor, tokens: Option
                        ignore_index: int = -100) -> torch.Tensor:
     """rf_token_logprobs_bwd: d(sum g_logp logp + sum g_entropy H) / d(logits) in the logits' type, from the
     forward's stats (and its entropy, with g_entropy)."""
-    lib = _lib.load()
-    ld = _logit_rows("token_logprobs_bwd", logits, inv_temp)
-    M, N = logits.shape
+    rows = _logit_rows("token_logprobs_bwd", logits, inv_temp)
+    M = rows[1]
     f32 = torch.float32
     ids, C = None, 0
     if tokens is not None and g_logp is not None:
         if g_logp.shape != tokens.shape:
             raise ValueError(f"token_logprobs_bwd: g_logp {tuple(g_logp.shape)} for tokens {tuple(tokens.shape)}")
-        ids = _row_list("token_logprobs_bwd: tokens", tokens.reshape(M, -1) if M else tokens.reshape(0, 1), logits)
+        ids = _token_ids("token_logprobs_bwd: tokens", tokens, logits)
         C = ids.shape[1]
-        g_logp = _row_list("token_logprobs_bwd: g_logp", g_logp.reshape(ids.shape), logits, f32)
+        g_logp = _row_list("token_logprobs_bwd: g_logp", g_logp.unsqueeze(1) if g_logp.dim() == 1 else g_logp, logits,
+                           f32)
     if g_entropy is not None:
         for t in (g_entropy, entropy):
-            if t is None or tuple(t.shape) != (M,) or t.device != logits.device:
+            if t is None or tuple(t.shape) != (M,) or t.get_device() != logits.get_device():
                 raise ValueError("token_logprobs_bwd: entropy and g_entropy are (M,) beside the logits")
         g_entropy, entropy = g_entropy.to(f32).contiguous(), entropy.to(f32).contiguous()
-    if tuple(stats.shape) != (M, 4) or stats.dtype != f32 or not stats.is_contiguous() or stats.device != logits.device:
-        raise ValueError("token_logprobs_bwd: stats is the forward's (M, 4) fp32")
-    out, ldd = _like_rows(logits, ld)
-    _run(lib.rf_token_logprobs_bwd, "rf_token_logprobs_bwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
-         float(inv_temp), _p(stats), _p(ids), C, int(ignore_index), _p(g_logp) if C else None, _p(entropy),
-         _p(g_entropy), _p(out), ldd)
+    _row_stats("token_logprobs_bwd", stats, logits)
+    return _logprobs_grad(rows, logits, stats, ids, C, int(ignore_index), g_logp if C else None, entropy, g_entropy)
+
+
+def _logprobs_grad(rows, logits, stats, ids, C: int, ignore: int, g_logp, entropy, g_entropy) -> torch.Tensor:
+    """The checked call; rows: _logit_rows of these logits."""
+    out, ldd = _like_rows(logits, rows[4])
+    _run(_lib.load().rf_token_logprobs_bwd, "rf_token_logprobs_bwd", logits, *rows, _p(stats), _p(ids), C, ignore,
+         _p(g_logp), _p(entropy), _p(g_entropy), _p(out), ldd)
     return out
+
+
+def _row_stats(what: str, stats: torch.Tensor, logits: torch.Tensor) -> None:
+    if (tuple(stats.shape) != (logits.shape[0], 4) or stats.dtype != torch.float32 or not stats.is_contiguous()
+            or stats.get_device() != logits.get_device()):
+        raise ValueError(f"{what}: stats is the forward's (M, 4) fp32")
 
 
 def _teacher(what: str, logits, teacher_logits, teacher_ids):
@@ -1115,20 +1134,25 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
     """rf_topk_distill_fwd: per row KL(q || p), q = softmax(teacher_logits * inv_temp) over the listed
     teacher_ids ((M, K <= 1024); id -1 or logit -inf: slot not used), p = softmax(logits * inv_temp) over all
     columns. Returns (rows (M,), stats (M, 4), loss, coef): loss = scale * sum(rows) / n and coef = scale / n,
-    one-element device tensors, with n the rows that use a slot (nan if none does). teacher_logits may be log probabilities."""
+    one-element device tensors, with n the rows that use a slot (nan if none does). teacher_logits may be
+    log probabilities."""
+    rows = _logit_rows("topk_distill", logits, inv_temp)
+    return _distill(rows, logits, *_teacher("topk_distill", logits, teacher_logits, teacher_ids), scale)
+
+
+def _distill(rows, logits, val, ids, scale: float):
+    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them."""
     lib = _lib.load()
-    ld = _logit_rows("topk_distill", logits, inv_temp)
-    M, N = logits.shape
-    val, ids = _teacher("topk_distill", logits, teacher_logits, teacher_ids)
-    dev = logits.device
-    rows = torch.empty(M, dtype=torch.float32, device=dev)
-    stats = torch.empty(M, 4, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    coef = torch.empty((), dtype=torch.float32, device=dev)
-    ws = _logprobs_ws(lib, logits, 0)
-    _run(lib.rf_topk_distill_fwd, "rf_topk_distill_fwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
-         float(inv_temp), _p(val), _p(ids), ids.shape[1], float(scale), _p(rows), _p(stats), _p(loss), _p(coef), _p(ws))
-    return rows, stats, loss, coef
+    code, M, N = rows[:3]
+    dev, f32 = logits.device, torch.float32
+    per_row = torch.empty(M, dtype=f32, device=dev)
+    stats = torch.empty(M, 4, dtype=f32, device=dev)
+    loss = torch.empty((), dtype=f32, device=dev)
+    coef = torch.empty((), dtype=f32, device=dev)
+    ws = _logprobs_ws(lib, code, M, N, 0, dev)
+    _run(lib.rf_topk_distill_fwd, "rf_topk_distill_fwd", logits, *rows, _p(val), _p(ids), ids.shape[1], float(scale),
+         _p(per_row), _p(stats), _p(loss), _p(coef), _p(ws))
+    return per_row, stats, loss, coef
 
 
 def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: torch.Tensor,
@@ -1136,18 +1160,20 @@ def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: 
                      inv_temp: float = 1.0) -> torch.Tensor:
     """rf_topk_distill_bwd: the gradient of g * coef * sum(rows) in the logits' type; g and coef one-element
     fp32 device tensors (the upstream gradient and the forward's coef)."""
-    lib = _lib.load()
-    ld = _logit_rows("topk_distill_bwd", logits, inv_temp)
-    M, N = logits.shape
+    rows = _logit_rows("topk_distill_bwd", logits, inv_temp)
     val, ids = _teacher("topk_distill_bwd", logits, teacher_logits, teacher_ids)
-    if tuple(stats.shape) != (M, 4) or stats.dtype != torch.float32 or not stats.is_contiguous():
-        raise ValueError("topk_distill_bwd: stats is the forward's (M, 4) fp32")
+    _row_stats("topk_distill_bwd", stats, logits)
     for t in (g, coef):
-        if t.numel() != 1 or t.dtype != torch.float32 or t.device != logits.device:
+        if t.numel() != 1 or t.dtype != torch.float32 or t.get_device() != logits.get_device():
             raise ValueError("topk_distill_bwd: g and coef are one-element fp32 tensors beside the logits")
-    out, ldd = _like_rows(logits, ld)
-    _run(lib.rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, dtype_code(logits.dtype), M, N, _p(logits), ld,
-         float(inv_temp), _p(stats), _p(val), _p(ids), ids.shape[1], _p(g), _p(coef), _p(out), ldd)
+    return _distill_grad(rows, logits, stats, val, ids, g, coef)
+
+
+def _distill_grad(rows, logits, stats, val, ids, g, coef) -> torch.Tensor:
+    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them."""
+    out, ldd = _like_rows(logits, rows[4])
+    _run(_lib.load().rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, *rows, stats.data_ptr(), val.data_ptr(),
+         ids.data_ptr(), ids.shape[1], g.data_ptr(), coef.data_ptr(), out.data_ptr(), ldd)
     return out
 
 

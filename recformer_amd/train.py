@@ -528,7 +528,6 @@ class _TokenLogprobs(torch.autograd.Function):
         return r.logp, r.entropy
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g_logp, g_entropy):
         if not ctx.needs_input_grad[0] or (g_logp is None and g_entropy is None):
             return None, None, None, None
@@ -543,18 +542,21 @@ class _TopkDistill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_ids, temp: float):
-        _, stats, loss, coef = ops.topk_distill(logits, teacher_logits, teacher_ids, 1.0 / temp, temp * temp)
-        ctx.save_for_backward(logits, teacher_logits, teacher_ids, stats, coef)
-        ctx.temp = temp
+        rows = ops._logit_rows("topk_distill_train", logits, 1.0 / temp)
+        val, ids = ops._teacher("topk_distill_train", logits, teacher_logits, teacher_ids)
+        _, stats, loss, coef = ops._distill(rows, logits, val, ids, temp * temp)
+        ctx.save_for_backward(logits, val, ids, stats, coef)
+        ctx.rows = rows
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
-        logits, tl, ti, stats, coef = ctx.saved_tensors
-        return ops.topk_distill_bwd(logits, stats, tl, ti, g.float(), coef, 1.0 / ctx.temp), None, None, None
+        logits, val, ids, stats, coef = ctx.saved_tensors
+        code, M, N, _, ld, inv_temp = ctx.rows
+        return (ops._distill_grad((code, M, N, logits.data_ptr(), ld, inv_temp), logits, stats, val, ids, g, coef),
+                None, None, None)
 
 
 def token_logprobs_train(logits: torch.Tensor, tokens: torch.Tensor, inv_temp: float = 1.0, ignore_index: int = -100):
@@ -569,7 +571,7 @@ def topk_distill_train(logits: torch.Tensor, teacher_logits: torch.Tensor, teach
     (ops.topk_distill). The factor keeps the gradient's size independent of temp."""
     if not temp > 0:
         raise ValueError(f"topk_distill_train: temperature {temp} must be positive")
-    return _TopkDistill.apply(logits, teacher_logits.detach(), teacher_ids, float(temp))
+    return _TopkDistill.apply(logits, teacher_logits, teacher_ids, float(temp))
 
 
 class _LMHeadTransform(torch.autograd.Function):
