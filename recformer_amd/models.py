@@ -798,6 +798,24 @@ class RecformerForSeqRec(nn.Module):
             return ops.cos_scores(z, table, inv_t, items_rnorm=rnorm)
         return ops.cos_scores_cand(z, table, candidates, inv_t, items_rnorm=rnorm)
 
+    @torch.no_grad()
+    def item_logprobs(self, pooler_output, items=None, k: int = 0, seen=None, want_entropy: bool = False):
+        """What the model answers for pooled vectors (B, d), as probabilities over the catalog: log probabilities
+        of the given items ((B,) or (B, C) ids) and the k best items under softmax(cos / temp)
+        (ops.token_logprobs). seen: (B, S) item ids to leave out of it (a user's history; -1: none)."""
+        scores = self.similarity_score(pooler_output)
+        if seen is not None:
+            # amin: a slot of -1 leaves column 0 as it is, whatever another slot says of it
+            mask = torch.full(seen.shape, float("-inf"), device=scores.device).masked_fill_(seen < 0, float("inf"))
+            scores = scores.scatter_reduce(1, seen.clamp_min(0), mask, "amin")
+        return ops.token_logprobs(scores, items, k=k, want_entropy=want_entropy)
+
+    def distill_loss(self, teacher_logits, teacher_ids, distill_temp: float = 1.0, **batch):
+        """Loss of the batch's catalog scores against a teacher's best items (train.topk_distill_train):
+        teacher_ids (B, K) with their logits or log probabilities (as a teacher's item_logprobs gives them)."""
+        from . import train
+        return train.topk_distill_train(self(**batch), teacher_logits, teacher_ids, distill_temp)
+
     def forward(self, input_ids=None, attention_mask=None, global_attention_mask=None, head_mask=None,
                 token_type_ids=None, position_ids=None, item_position_ids=None, inputs_embeds=None,
                 output_attentions=None, output_hidden_states=None, return_dict=None, candidates=None,
@@ -893,6 +911,12 @@ class RecformerForPretraining(nn.Module):
         t = ops.gemm(x, w["w_d"], w["b_d"], ops.RF_EPI_BIAS_GELU)
         t = ops.layernorm(t, w["ln_w"], w["ln_b"], self.config.layer_norm_eps)
         return ops.gemm(t, w["w_dec"], w["b_dec"], ops.RF_EPI_BIAS)
+
+    @torch.no_grad()
+    def token_logprobs(self, hidden: torch.Tensor, tokens=None, k: int = 0, want_entropy: bool = False):
+        """What the masked-LM head says of (M, d) hidden rows: log probabilities of the given words ((M,) or
+        (M, C) ids, -100: none) and the k best words (ops.token_logprobs on lm_logits)."""
+        return ops.token_logprobs(self.lm_logits(hidden), tokens, k=k, want_entropy=want_entropy)
 
     def forward(self, input_ids_a=None, attention_mask_a=None, global_attention_mask_a=None,
                 token_type_ids_a=None, item_position_ids_a=None, mlm_input_ids_a=None, mlm_labels_a=None,

@@ -417,3 +417,52 @@ def test_refusals(dev):
         train.topk_distill_train(x, torch.zeros(4, 2, device=dev), torch.zeros(4, 2, dtype=torch.long, device=dev), 0.0)
     with pytest.raises(ValueError):
         ops.token_logprobs_bwd(x, torch.zeros(4, 3, device=dev), tok, torch.ones(4, device=dev))
+
+
+def test_model_answers_and_learns_from_a_teacher(dev):
+    """RecformerForSeqRec.item_logprobs / distill_loss and RecformerForPretraining.token_logprobs: the numbers of
+    the scores they come from, a history left out, and parameter gradients equal to autograd's through the
+    plain formula on the same scores (the backward below the scores is the same: 1e-5 of the largest, from
+    the 2e-5 of the scores' gradients)."""
+    from recformer_amd.hashinit import hash_tensor
+    from recformer_amd.models import RecformerForSeqRec
+    from recformer_amd.synth import C1, synth_batch
+    from tests.common import hashed_model, hashed_pretrain
+    m = hashed_model(dict(C1, item_num=300), 1, RecformerForSeqRec)
+    m.init_item_embedding(hash_tensor("items", (300, C1["hidden_size"]), "weight", std=1.0))
+    m = m.to(dev)
+    batch = {k: v.to(dev) for k, v in synth_batch(4, 96, C1["vocab_size"], seed=1).items()}
+    with torch.no_grad():
+        z = m.longformer(**batch).pooler_output
+        scores = m.similarity_score(z)
+    seen = torch.tensor([[3, 5], [0, -1], [-1, -1], [7, 7]], device=dev)
+    r = m.item_logprobs(z, torch.tensor([3, 1, 2, 9], device=dev), k=10, seen=seen, want_entropy=True)
+    masked = scores.clone()
+    masked[0, [3, 5]] = -INF
+    masked[1, 0] = -INF
+    masked[3, 7] = -INF
+    logp, _, h = ref_softmax(masked, 1.0)
+    close_logp(r.logp, logp[torch.arange(4), [3, 1, 2, 9]])
+    check_top(masked, r, 10, 1.0)
+    teacher = ops.token_logprobs(torch.randn(4, 300, device=dev), k=20)
+    loss = m.distill_loss(teacher.top_logp, teacher.top_ids, 2.0, **batch)
+    loss.backward()
+    got = {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
+    assert got
+    m.zero_grad(set_to_none=True)
+    s = m(**batch)
+    ls = torch.log_softmax(s.double() / 2.0, 1)
+    lq = torch.log_softmax(teacher.top_logp.double() / 2.0, 1)
+    plain = 4.0 * (lq.exp() * (lq - ls.gather(1, teacher.top_ids))).sum(1).mean()
+    assert abs(float(plain.detach()) - float(loss.detach())) <= 4.0 * 2e-5 * 40
+    plain.backward()
+    for n, g in got.items():
+        w = dict(m.named_parameters())[n].grad
+        assert float((g - w).abs().max()) <= 1e-3 * float(w.abs().max()) + 1e-9, n
+    lm = hashed_pretrain(C1).to(dev)
+    hidden = torch.randn(5, C1["hidden_size"], device=dev)
+    words = torch.tensor([1, 2, -100, 4, 5], device=dev)
+    r = lm.token_logprobs(hidden, words, k=3)
+    logits = lm.lm_logits(hidden)
+    close_logp(r.logp, torch.where(words < 0, 0.0, ref_softmax(logits, 1.0)[0].gather(1, words.clamp_min(0)[:, None])[:, 0]))
+    check_top(logits, r, 3, 1.0)

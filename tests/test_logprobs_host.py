@@ -1,0 +1,122 @@
+"""Refusals of the log-probability, distillation and 4-bit entry points that need no device: each comes back as
+an error with a message before anything is launched, and calls on nothing succeed."""
+import ctypes
+
+import pytest
+import torch
+
+from recformer_amd import Mxfp4Catalog, _lib, ops, train
+
+A = 1 << 12  # an address that is never read
+
+
+def err(rc):
+    assert rc != 0
+    return _lib.load().rf_last_error().decode()
+
+
+def fwd(dtype=0, M=2, N=50, x=A, ld=50, it=1.0, tok=A, C=1, k=0, logp=A, ent=None, tv=None, ti=None, st=None, ws=None):
+    return _lib.load().rf_token_logprobs_fwd(dtype, M, N, x, ld, it, tok, C, -100, k, logp, ent, tv, ti, st, ws, None)
+
+
+def test_token_logprobs_refusals():
+    assert "dtype" in err(fwd(dtype=7))
+    assert "shape" in err(fwd(N=0))
+    assert "shape" in err(fwd(ld=49))
+    for it in (0.0, -1.0, float("nan"), float("inf")):
+        assert "temperature" in err(fwd(it=it))
+    assert "entries" in err(fwd(C=1025))
+    for k in (51, 257, -1):
+        assert "k=" in err(fwd(N=300 if k == 257 else 50, ld=300, k=k, tv=A, ti=A))
+    assert "null" in err(fwd(x=None))
+    assert "null" in err(fwd(tok=None))
+    assert "null" in err(fwd(k=3))
+    assert "misaligned" in err(fwd(x=A + 2))
+    assert "workspace" in err(fwd(M=1, N=1 << 20, ld=1 << 20))
+    assert "workspace" in err(fwd(M=1, N=1 << 20, ld=1 << 20, ws=A + 8))
+    assert fwd(M=0) == 0
+
+
+def test_gradient_refusals():
+    lib = _lib.load()
+
+    def bwd(x=A, ld=56, st=A, tok=A, g=A, ent=None, ge=None, d=A + 64, ldd=56):
+        return lib.rf_token_logprobs_bwd(1, 2, 50, x, ld, 1.0, st, tok, 1, -100, g, ent, ge, d, ldd, None)
+
+    assert "entropy" in err(bwd(ge=A))
+    assert "aligned" in err(bwd(d=A + 66))
+    assert "aligned" in err(bwd(ldd=51))
+    assert "null" in err(bwd(st=None))
+    assert "shape" in err(bwd(ldd=48))
+
+    def dist(K=2, t=A, rows=A, st=A, loss=None, coef=None):
+        return lib.rf_topk_distill_fwd(0, 2, 50, A, 50, 1.0, t, A, K, 1.0, rows, st, loss, coef, None, None)
+
+    assert "K=0" in err(dist(K=0))
+    assert "entries" in err(dist(K=1025))
+    assert "null" in err(dist(t=None))
+    assert "together" in err(dist(loss=A))
+    assert "null" in err(lib.rf_topk_distill_bwd(0, 2, 50, A, 50, 1.0, A, A, A, 2, None, A, A, 50, None))
+
+
+def test_workspace_sizes():
+    lib = _lib.load()
+    assert lib.rf_logprobs_workspace(1, 4915, 50265, 20) == 0  # a row a workgroup
+    assert lib.rf_logprobs_workspace(0, 0, 50, 5) == 0
+    n = lib.rf_logprobs_workspace(0, 1, 1000003, 256)
+    assert n > 0 and n % (16 + 8 * 256) == 0
+    # a row of 2^31 - 17 columns still has a plan
+    assert lib.rf_logprobs_workspace(0, 1, 2 ** 31 - 17, 256) >= (2 ** 31 // 32768) * (16 + 8 * 256)
+
+
+def test_mxfp4_refusals():
+    lib = _lib.load()
+    assert "dtype" in err(lib.rf_mxfp4_quantize(3, 1, 32, A, 32, 1e-8, A, A, None, None))
+    assert "shape" in err(lib.rf_mxfp4_quantize(0, 1, 0, A, 32, 1e-8, A, A, None, None))
+    assert "shape" in err(lib.rf_mxfp4_quantize(0, 1, 32, A, 31, 1e-8, A, A, None, None))
+    assert "misaligned" in err(lib.rf_mxfp4_quantize(0, 1, 32, A, 32, 1e-8, A + 4, A, None, None))
+    assert "null" in err(lib.rf_mxfp4_quantize(0, 1, 32, None, 32, 1e-8, A, A, None, None))
+    assert "shape" in err(lib.rf_mxfp4_dequantize(0, 1, 32, A, A, A, 31, None))
+
+    def gemm(M=2, N=8, K=32, ac=A, ra=None, rw=None, bias=None, C=A, ldc=8, dt=0):
+        return lib.rf_mxfp4_gemm(dt, M, N, K, ac, A, A, A, bias, ra, rw, 1.0, C, ldc, None)
+
+    assert "together" in err(gemm(ra=A))
+    assert "aligned" in err(gemm(ac=A + 8))
+    assert "aligned" in err(gemm(C=A + 4))
+    assert "aligned" in err(gemm(ldc=9))
+    assert "aligned" in err(gemm(bias=A + 4))
+    assert "shape" in err(gemm(ldc=7))
+    assert "64 MB" in err(gemm(ldc=1 << 25))
+    assert gemm(M=0) == 0 and gemm(N=0) == 0
+
+
+def test_tensors_on_the_cpu_are_refused():
+    x, ids = torch.zeros(2, 64), torch.zeros(2, dtype=torch.long)
+    q = ops.Mxfp4(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 64)
+    assert q.rows == 2
+    for call in (lambda: ops.token_logprobs(x, ids), lambda: train.token_logprobs_train(x, ids),
+                 lambda: train.topk_distill_train(x, x, ids[:, None]), lambda: ops.mxfp4_quantize(x),
+                 lambda: ops.mxfp4_dequantize(q), lambda: ops.mxfp4_gemm(x, q), lambda: Mxfp4Catalog.from_items(x),
+                 lambda: Mxfp4Catalog(q, torch.ones(2)).scores(x, 1.0)):
+        with pytest.raises(_lib.RecformerHipError):
+            call()
+    with pytest.raises(ValueError):
+        Mxfp4Catalog(q, torch.ones(3))
+
+
+def test_signatures_take_what_the_header_declares():
+    """The argument counts of the new entry points, header against binding."""
+    import os
+    import re
+    txt = open(os.path.join(os.path.dirname(__file__), "..", "include", "recformer_hip.h")).read()
+    for name in ("rf_token_logprobs_fwd", "rf_token_logprobs_bwd", "rf_topk_distill_fwd", "rf_topk_distill_bwd",
+                 "rf_logprobs_workspace", "rf_mxfp4_quantize", "rf_mxfp4_dequantize", "rf_mxfp4_gemm"):
+        args = re.search(name + r"\(([^;]*)\);", txt).group(1).split(",")
+        types = _lib.SIGNATURES[name][1]
+        assert len(args) == len(types), name
+        for a, t in zip(args, types):
+            ptr = "*" in a or "rf_stream_t" in a
+            want = (ctypes.c_void_p if ptr else ctypes.c_float if "float" in a else
+                    ctypes.c_int64 if "int64_t" in a else ctypes.c_int)
+            assert t is want, (name, a)
