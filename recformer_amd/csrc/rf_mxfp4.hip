@@ -93,33 +93,45 @@ __device__ __forceinline__ float scale_value(int s) {  // 2^(s - 127); 255: NaN
   return __uint_as_float(s == 255 ? 0x7FC00000u : s == 0 ? 0x00400000u : (uint32_t)s << 23);
 }
 
+// Eights of values, flat over the rows (G = ceil(K / 8) a row), two a thread 64 apart so that a wave's loads and
+// stores are contiguous. HBM bound.
 template <typename T>
-__global__ void __launch_bounds__(256) k_mxfp4_dequantize(int64_t M, int K, int KB, const uint8_t* __restrict__ codes,
+__global__ void __launch_bounds__(256) k_mxfp4_dequantize(int64_t total, int G, int K, int KB,
+                                                          const uint8_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ scales, T* __restrict__ out,
-                                                          int64_t ldo, int sh, bool vec) {
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = gid >> sh;
-  const int L = 1 << sh, sub = (int)(gid & (L - 1));
-  if (row >= M) return;
-  T* o = out + row * ldo;
-  for (int c = 8 * sub; c < K; c += 8 * L) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + row * KB * 16 + (c >> 1));
-    const float f = scale_value(scales[row * KB + (c >> 5)]);
+                                                          int64_t ldo, bool vec) {
+  const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 128 + (threadIdx.x & 63);
+  int64_t row[2];
+  int c[2];
+  uint32_t w[2];
+  int sc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t at = min(first + 64 * i, total - 1);
+    row[i] = total <= 0xFFFFFFFFll ? (int64_t)((uint32_t)at / (uint32_t)G) : at / G;
+    c[i] = (int)(at - row[i] * G) * 8;
+    w[i] = *reinterpret_cast<const uint32_t*>(codes + row[i] * KB * 16 + (c[i] >> 1));
+    sc[i] = scales[row[i] * KB + (c[i] >> 5)];
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (first + 64 * i >= total) break;
+    const float f = scale_value(sc[i]);
+    typedef float v2 __attribute__((ext_vector_type(2)));
+    const v2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 0),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 1),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 2),
+                     __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 3)};
     T e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t q = w >> (4 * i);
-      // magnitude code m: 0 0.5 | 1 1.5 | 2 3 | 4 6 = (1 + (m & 1) / 2) 2^((m >> 1) - 1), and m / 2 below 2
-      const uint32_t m = q & 7;
-      const float a = m < 2 ? 0.5f * (float)m : __uint_as_float((126 + (m >> 1)) << 23 | (m & 1) << 22);
-      e[i] = from_f32<T>((q & 8 ? -a : a) * f);
-    }
-    if (vec && c + 8 <= K) {
-      __builtin_memcpy(__builtin_assume_aligned(o + c, 16), e, sizeof(e));
+    for (int x = 0; x < 8; ++x) e[x] = from_f32<T>(p[x >> 1][x & 1] * f);
+    T* o = out + row[i] * ldo + c[i];
+    if (vec && c[i] + 8 <= K) {
+      __builtin_memcpy(__builtin_assume_aligned(o, 16), e, sizeof(e));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < K) o[c + i] = e[i];
+      for (int x = 0; x < 8; ++x)
+        if (c[i] + x < K) o[x] = e[x];
     }
   }
 }
@@ -482,53 +494,102 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
   wait_vm<0>();  // the last stage's (empty) loads land before the LDS is given away
 }
 
-// Up to 16 MT rows of A: W is read once from memory straight into the fragments, a wave per 16 of its rows,
-// U steps of K at a time in flight; the A rows come from the caches. Bound by the read of W.
-template <typename T, int MT>
+// Up to 16 MT rows of A: W is read once from memory straight into the fragments, a wave per 16 NT of its rows,
+// U steps of K in flight; the A rows come from the caches. Bound by the read of W. DW: a row's four scales of
+// a step are one word; the four lanes of a row load the words of four steps and trade them (a byte a lane and
+// step took 66 instead of 41 us at 1 x 100000 x 4096).
+template <typename T, int MT, int NT, bool DW>
 __global__ void __launch_bounds__(256) k_mxfp4_skinny(MxArgs a) {
-  constexpr int U = MT == 1 ? 6 : MT == 2 ? 4 : 2;
+  constexpr int U = NT == 4 ? (MT == 4 ? 1 : 2) : MT == 4 ? 2 : 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
-  const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * 16;
+  const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * (16 * NT);
   if (n0 >= a.N) return;
   const int KB = a.KB, nk = (KB + 3) >> 2;
-  const int64_t wr = min(n0 + r, a.N - 1);
-  const uint8_t *wc = a.wc + wr * KB * 16, *ws = a.ws + wr * KB;
-  f32x4 acc[MT];
+  const uint8_t *wc[NT], *ws[NT], *ac[MT], *as[MT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < nk; k0 += U) {
-    u32x4 fw[U];
-    uint32_t sw[U];
+  for (int i = 0; i < NT; ++i) {
+    const int64_t row = min(n0 + i * 16 + r, a.N - 1);
+    wc[i] = a.wc + row * KB * 16;
+    ws[i] = a.ws + row * KB;
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int b = min(4 * (k0 + u) + g, KB - 1);
-      fw[u] = *reinterpret_cast<const u32x4*>(wc + b * 16);
-      sw[u] = ws[b];
+  for (int j = 0; j < MT; ++j) {
+    const int64_t row = min((int64_t)j * 16 + r, a.M - 1);
+    ac[j] = a.ac + row * KB * 16;
+    as[j] = a.as + row * KB;
+  }
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto words = [&](const uint8_t* p, int k4) -> uint32_t {  // of step k4 + g
+    return *reinterpret_cast<const uint32_t*>(p + 4 * min(k4 + g, nk - 1));
+  };
+  for (int k4 = 0; k4 < nk; k4 += 4) {
+    uint32_t w4[NT], a4[MT];
+    if (DW) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) w4[i] = words(ws[i], k4);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) a4[j] = words(as[j], k4);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int b = 4 * (k0 + u) + g;
-      const bool in = b < KB;
-      const uint32_t sb = in ? sw[u] : 127;
+    for (int k0 = 0; k0 < 4; k0 += U) {
+      if (k4 + k0 >= nk) break;
+      u32x4 fw[U][NT], fa[U][MT];
+      uint32_t sw[U][NT], sa[U][MT];
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int64_t m = min((int64_t)j * 16 + r, a.M - 1);
-        u32x4 fa = *reinterpret_cast<const u32x4*>(a.ac + m * KB * 16 + min(b, KB - 1) * 16);
-        uint32_t sa = a.as[m * KB + min(b, KB - 1)];
-        if (!in) {
-          fa = u32x4{0, 0, 0, 0};
-          sa = 127;
+      for (int u = 0; u < U; ++u) {
+        const int b = min(4 * (k4 + k0 + u) + g, KB - 1);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          fw[u][i] = *reinterpret_cast<const u32x4*>(wc[i] + b * 16);
+          if (!DW) sw[u][i] = ws[i][b];
         }
-        acc[j] = mfma_mx(fw[u], fa, acc[j], sb, sa);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          fa[u][j] = *reinterpret_cast<const u32x4*>(ac[j] + b * 16);
+          if (!DW) sa[u][j] = as[j][b];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (DW) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i) sw[u][i] = (uint32_t)__shfl((int)w4[i], r + 16 * (k0 + u), 64) >> (8 * g);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) sa[u][j] = (uint32_t)__shfl((int)a4[j], r + 16 * (k0 + u), 64) >> (8 * g);
+        }
+        if (4 * (k4 + k0 + u) + 4 > KB) {  // past the last block: 0 * 1
+          const bool in = 4 * (k4 + k0 + u) + g < KB;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) sw[u][i] = in ? sw[u][i] : 127;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            sa[u][j] = in ? sa[u][j] : 127;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) fa[u][j][x] = in ? fa[u][j][x] : 0;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) acc[i][j] = mfma_mx(fw[u][i], fa[u][j], acc[i][j], sw[u][i], sa[u][j]);
       }
     }
   }
-  const int64_t n = n0 + 4 * g;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int64_t m = (int64_t)j * 16 + r;
-    if (m < a.M && n < a.N) store4<T>(a, m, n, acc[j], a.ra ? a.ra[m] * a.col_scale : 1.f, cols_of(a, n));
+  for (int i = 0; i < NT; ++i) {
+    const int64_t n = n0 + i * 16 + 4 * g;
+    if (n >= a.N) continue;
+    const Cols c = cols_of(a, n);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const int64_t m = (int64_t)j * 16 + r;
+      if (m < a.M) store4<T>(a, m, n, acc[i][j], a.ra ? a.ra[m] * a.col_scale : 1.f, c);
+    }
   }
 }
 
@@ -539,25 +600,21 @@ static int lane_shift(int K) {  // lanes a row: enough for its eights, at least 
   return sh;
 }
 
-template <typename T>
+template <typename T, int MT, bool DW>
+static void launch_skinny(const MxArgs& a, hipStream_t st) {
+  // four row tiles a wave share the A fragments; one where that would leave CUs without waves
+  if (a.N >= 64 * 4 * 512) k_mxfp4_skinny<T, MT, 4, DW><<<(unsigned)((a.N + 255) / 256), 256, 0, st>>>(a);
+  else k_mxfp4_skinny<T, MT, 1, DW><<<(unsigned)((a.N + 63) / 64), 256, 0, st>>>(a);
+}
+
+template <typename T, bool DW>
 static void launch_gemm(const MxArgs& a, hipStream_t st) {
-  if (a.M <= 64) {
-    const unsigned grid = (unsigned)((a.N + 63) / 64);
-    if (a.M <= 16) k_mxfp4_skinny<T, 1><<<grid, 256, 0, st>>>(a);
-    else if (a.M <= 32) k_mxfp4_skinny<T, 2><<<grid, 256, 0, st>>>(a);
-    else k_mxfp4_skinny<T, 4><<<grid, 256, 0, st>>>(a);
-  } else {
-    const unsigned grid = (unsigned)std::min(a.nTm * a.nTn, MX_WGS);
-    const bool dw = a.KB % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.as) | reinterpret_cast<uintptr_t>(a.ws)) & 3) == 0;
-    constexpr int lds = 2 * MX_STAGE;
-    if (dw) {
-      (void)hipFuncSetAttribute((const void*)k_mxfp4_gemm<T, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-      k_mxfp4_gemm<T, true><<<grid, 256, lds, st>>>(a);
-    } else {
-      (void)hipFuncSetAttribute((const void*)k_mxfp4_gemm<T, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-      k_mxfp4_gemm<T, false><<<grid, 256, lds, st>>>(a);
-    }
-  }
+  if (a.M <= 16) return launch_skinny<T, 1, DW>(a, st);
+  if (a.M <= 32) return launch_skinny<T, 2, DW>(a, st);
+  if (a.M <= 64) return launch_skinny<T, 4, DW>(a, st);
+  constexpr int lds = 2 * MX_STAGE;
+  (void)hipFuncSetAttribute((const void*)k_mxfp4_gemm<T, DW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  k_mxfp4_gemm<T, DW><<<(unsigned)std::min(a.nTm * a.nTn, MX_WGS), 256, lds, st>>>(a);
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -598,12 +655,13 @@ extern "C" int rf_mxfp4_dequantize(int dtype, int M, int K, const uint8_t* codes
   const int es = dtype == RF_F32 ? 4 : 2;
   RF_REQUIRE((reinterpret_cast<uintptr_t>(out) & (es - 1)) == 0 && aligned16(codes),
              "rf_mxfp4_dequantize: misaligned rows or codes");
-  const int KB = (K + 31) / 32, sh = lane_shift(K);
+  const int KB = (K + 31) / 32, G = (K + 7) / 8;
   const bool vec = aligned16(out) && ldo * es % 16 == 0;
-  const int64_t blocks = (((int64_t)M << sh) + 255) / 256;
+  const int64_t total = (int64_t)M * G, blocks = (total + 511) / 512;
   RF_REQUIRE(blocks < 0x7FFFFFFF, "rf_mxfp4_dequantize: too many rows");
   hipStream_t st = as_stream(stream);
-#define MXD(T) k_mxfp4_dequantize<T><<<(unsigned)blocks, 256, 0, st>>>(M, K, KB, codes, scales, (T*)out, ldo, sh, vec)
+#define MXD(T) \
+  k_mxfp4_dequantize<T><<<(unsigned)blocks, 256, 0, st>>>(total, G, K, KB, codes, scales, (T*)out, ldo, vec)
   if (dtype == RF_F32) MXD(float);
   else if (dtype == RF_BF16) MXD(bf16);
   else MXD(f16);
@@ -639,8 +697,11 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
   a.gn = 4;  // column tiles side by side: 1 to 32 took within 3% of each other
   RF_REQUIRE((int64_t)a.nTm * a.nTn < 0x7FFFFFFF, "rf_mxfp4_gemm: too many tiles");
   hipStream_t st = as_stream(stream);
-  if (out_dtype == RF_F32) launch_gemm<float>(a, st);
-  else if (out_dtype == RF_BF16) launch_gemm<bf16>(a, st);
-  else launch_gemm<f16>(a, st);
+  const bool dw = a.KB % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.as) | reinterpret_cast<uintptr_t>(a.ws)) & 3) == 0;
+#define MXG(T) dw ? launch_gemm<T, true>(a, st) : launch_gemm<T, false>(a, st)
+  if (out_dtype == RF_F32) MXG(float);
+  else if (out_dtype == RF_BF16) MXG(bf16);
+  else MXG(f16);
+#undef MXG
   RF_LAUNCH_CHECK("rf_mxfp4_gemm");
 }
