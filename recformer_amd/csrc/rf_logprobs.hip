@@ -32,6 +32,8 @@ constexpr float LP_NINF = -__builtin_inff();
 constexpr int LP_R = 8;         // 16-byte chunks of a row per thread
 constexpr int LP_KMAX = 256;    // alternatives
 constexpr int LP_LIST = 1024;   // given entries / teacher entries per row
+constexpr int LP_NMAX = 0x7FFFFFFF - (1 << 16);  // columns: a workgroup's numbers past the end of a row fit 32 bits
+constexpr float LP_ITMAX = 2e38f;                // it log2(e) is finite
 
 // ---- elements of a row -----------------------------------------------------------------------
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -708,7 +710,7 @@ static void lp_plan(int dtype, int M, int N, int k, int* S, int* cps) {
   const int V = lp_vec(dtype);
   const int64_t nch = ((int64_t)N + 2 * V - 2) / V;  // of a row that starts anywhere in a chunk
   int64_t s = (nch + 1024 * LP_R - 1) / (1024 * LP_R);
-  const int64_t want = std::min({(int64_t)(2 * LP_CUS + M - 1) / M, nch / LP_MIN_CHUNKS,
+  const int64_t want = std::min({(2 * LP_CUS + (int64_t)M - 1) / M, nch / LP_MIN_CHUNKS,
                                  (int64_t)16384 / std::max(k, 16)});
   s = std::max(s, want);
   s = std::max<int64_t>(s, 1);
@@ -716,18 +718,21 @@ static void lp_plan(int dtype, int M, int N, int k, int* S, int* cps) {
   *S = (int)((nch + *cps - 1) / *cps);
 }
 
+// threads of a workgroup: one wave a row where rows are short and fill the card, 1024 where a slice needs them
+// or many alternatives want many groups, 256 otherwise
+static int lp_threads(const LpArgs& a) {
+  if (a.cps <= 64 * LP_R && a.S == 1 && a.M >= 2048 && a.k <= 16) return 64;
+  return a.cps <= 256 * LP_R && a.k <= 64 ? 256 : 1024;
+}
+
 template <typename T, bool ENT, bool TOP, bool TEACH>
 static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
   const T* p = (const T*)x;
   const unsigned grid = (unsigned)((int64_t)a.M * a.S);
-  // one wave a row where rows are short and fill the card; 1024 threads where a slice needs them or many
-  // alternatives want many groups
-  if (a.cps <= 64 * LP_R && a.S == 1 && a.M >= 2048 && a.k <= 16)
-    k_logprobs<T, 64, ENT, TOP, TEACH><<<grid, 64, 0, st>>>(a, p);
-  else if (a.cps <= 256 * LP_R && a.k <= 64)
-    k_logprobs<T, 256, ENT, TOP, TEACH><<<grid, 256, 0, st>>>(a, p);
-  else
-    k_logprobs<T, 1024, ENT, TOP, TEACH><<<grid, 1024, 0, st>>>(a, p);
+  const int tpb = lp_threads(a);
+  if (tpb == 64) k_logprobs<T, 64, ENT, TOP, TEACH><<<grid, 64, 0, st>>>(a, p);
+  else if (tpb == 256) k_logprobs<T, 256, ENT, TOP, TEACH><<<grid, 256, 0, st>>>(a, p);
+  else k_logprobs<T, 1024, ENT, TOP, TEACH><<<grid, 1024, 0, st>>>(a, p);
   if (a.S > 1) {
     if (!TOP || (a.S * a.k <= 2048 && a.k <= 64)) k_logprobs_join<T, 256, TOP, TEACH><<<a.M, 256, 0, st>>>(a, p);
     else k_logprobs_join<T, 1024, TOP, TEACH><<<a.M, 1024, 0, st>>>(a, p);
@@ -737,8 +742,9 @@ static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
 static int lp_forward(const char* name, int dtype, const LpArgs& in, const void* logits, void* ws, hipStream_t st) {
   LpArgs a = in;
   RF_REQUIRE(dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16, "%s: bad dtype %d", name, dtype);
-  RF_REQUIRE(a.M >= 0 && a.N > 0 && a.ld >= a.N, "%s: bad shape M=%d N=%d ld=%lld", name, a.M, a.N, (long long)a.ld);
-  RF_REQUIRE(a.it > 0.f && a.it <= 3e38f, "%s: inverse temperature %g must be positive and finite", name, a.it);
+  RF_REQUIRE(a.M >= 0 && a.N > 0 && a.N <= LP_NMAX && a.ld >= a.N, "%s: bad shape M=%d N=%d ld=%lld", name, a.M, a.N,
+             (long long)a.ld);
+  RF_REQUIRE(a.it > 0.f && a.it <= LP_ITMAX, "%s: inverse temperature %g must be positive and finite", name, a.it);
   RF_REQUIRE(a.nids >= 0 && a.nids <= LP_LIST, "%s: %d entries per row (0 to %d)", name, a.nids, LP_LIST);
   RF_REQUIRE(a.k >= 0 && a.k <= LP_KMAX && a.k <= a.N, "%s: k=%d must be in [0, min(N, %d)]", name, a.k, LP_KMAX);
   if (a.M == 0) return RF_OK;
@@ -746,7 +752,9 @@ static int lp_forward(const char* name, int dtype, const LpArgs& in, const void*
              "%s: null pointer", name);
   RF_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (dtype == RF_F32 ? 3 : 1)) == 0, "%s: misaligned logits", name);
   lp_plan(dtype, a.M, a.N, a.k, &a.S, &a.cps);
-  RF_REQUIRE((int64_t)a.M * a.S < 0x7FFFFFFF, "%s: %d rows of %d slices are too many", name, a.M, a.S);
+  const int tpb = lp_threads(a);
+  RF_REQUIRE((int64_t)a.M * a.S * tpb <= 0xFFFFFFFFll && (a.S == 1 || (int64_t)a.M * 1024 <= 0xFFFFFFFFll),
+             "%s: %d rows of %d slices are too many for a launch", name, a.M, a.S);
   if (a.S > 1) {
     RF_REQUIRE(ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0, "%s: workspace missing or not 16-byte aligned", name);
     a.part = (float*)ws;
@@ -770,8 +778,8 @@ static int lp_backward(const char* name, int dtype, const LpBwdArgs& in, const v
                        hipStream_t st) {
   LpBwdArgs a = in;
   RF_REQUIRE(dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16, "%s: bad dtype %d", name, dtype);
-  RF_REQUIRE(a.M >= 0 && a.N > 0 && a.ld >= a.N && a.ldd >= a.N, "%s: bad shape", name);
-  RF_REQUIRE(a.it > 0.f && a.it <= 3e38f, "%s: inverse temperature %g must be positive and finite", name, a.it);
+  RF_REQUIRE(a.M >= 0 && a.N > 0 && a.N <= LP_NMAX && a.ld >= a.N && a.ldd >= a.N, "%s: bad shape", name);
+  RF_REQUIRE(a.it > 0.f && a.it <= LP_ITMAX, "%s: inverse temperature %g must be positive and finite", name, a.it);
   RF_REQUIRE(a.nids >= 0 && a.nids <= LP_LIST, "%s: %d entries per row (0 to %d)", name, a.nids, LP_LIST);
   if (a.M == 0) return RF_OK;
   RF_REQUIRE(logits && dlogits && a.stats && (a.nids == 0 || a.ids), "%s: null pointer", name);
@@ -783,7 +791,8 @@ static int lp_backward(const char* name, int dtype, const LpBwdArgs& in, const v
   const int64_t nch = ((int64_t)a.N + 2 * V - 2) / V;
   a.S = (int)((nch + LB_TPB * LB_R - 1) / (LB_TPB * LB_R));
   a.cps = (int)((nch + a.S - 1) / a.S);
-  RF_REQUIRE((int64_t)a.M * a.S < 0x7FFFFFFF, "%s: %d rows of %d slices are too many", name, a.M, a.S);
+  RF_REQUIRE((int64_t)a.M * a.S * LB_TPB <= 0xFFFFFFFFll, "%s: %d rows of %d slices are too many for a launch", name,
+             a.M, a.S);
   const unsigned grid = (unsigned)((int64_t)a.M * a.S);
 #define LB_T(T)                                                                                        \
   if (a.g_ent) k_logprobs_bwd<T, true><<<grid, LB_TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits);       \

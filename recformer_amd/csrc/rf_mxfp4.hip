@@ -639,7 +639,7 @@ extern "C" int rf_mxfp4_quantize(int dtype, int M, int K, const void* x, int64_t
   const int KB = (K + 31) / 32, sh = lane_shift(K);
   const bool vec = aligned16(x) && ldx * es % 16 == 0;
   const int64_t blocks = (((int64_t)M << sh) + 255) / 256;
-  RF_REQUIRE(blocks < 0x7FFFFFFF, "rf_mxfp4_quantize: too many rows");
+  RF_REQUIRE(blocks * 256 <= 0xFFFFFFFFll, "rf_mxfp4_quantize: %d rows are too many for a launch", M);
   hipStream_t st = as_stream(stream);
 #define MXQ(T)                                                                                                      \
   k_mxfp4_quantize<T><<<(unsigned)blocks, 256, 0, st>>>(M, K, KB, (const T*)x, ldx, sh, vec, eps, codes, scales, rnorm)
@@ -662,7 +662,7 @@ extern "C" int rf_mxfp4_dequantize(int dtype, int M, int K, const uint8_t* codes
   const int KB = (K + 31) / 32, G = (K + 7) / 8;
   const bool vec = aligned16(out) && ldo * es % 16 == 0;
   const int64_t total = (int64_t)M * G, blocks = (total + 511) / 512;
-  RF_REQUIRE(blocks < 0x7FFFFFFF, "rf_mxfp4_dequantize: too many rows");
+  RF_REQUIRE(blocks * 256 <= 0xFFFFFFFFll, "rf_mxfp4_dequantize: %d rows are too many for a launch", M);
   hipStream_t st = as_stream(stream);
 #define MXD(T) \
   k_mxfp4_dequantize<T><<<(unsigned)blocks, 256, 0, st>>>(total, G, K, KB, codes, scales, (T*)out, ldo, vec)
@@ -699,7 +699,7 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
   // row tiles whose codes fill half of an XCD's 4 MB of L2
   a.gm = (int)std::max<int64_t>(1, std::min<int64_t>(a.nTm, (2 << 20) / ((int64_t)MX_T * a.KB * 16)));
   a.gn = 4;  // column tiles side by side: 1 to 32 took within 3% of each other
-  RF_REQUIRE((int64_t)a.nTm * a.nTn < 0x7FFFFFFF, "rf_mxfp4_gemm: too many tiles");
+  RF_REQUIRE((int64_t)a.nTm * a.nTn < 0x7FFFFFFF - MX_WGS, "rf_mxfp4_gemm: too many tiles");
   hipStream_t st = as_stream(stream);
   const bool dw = a.KB % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.as) | reinterpret_cast<uintptr_t>(a.ws)) & 3) == 0;
 #define MXG(T) dw ? launch_gemm<T, true>(a, st) : launch_gemm<T, false>(a, st)

@@ -1007,13 +1007,13 @@ def _logit_rows(what: str, logits: torch.Tensor, inv_temp: float):
     code = dtype_code(logits.dtype)
     ld = _rowmajor(logits, "logits")
     M, N = logits.shape
-    if N < 1 or N >= 2 ** 31 - 16 or M >= 2 ** 31:
+    if N < 1 or N >= 2 ** 31 - 2 ** 16 or M >= 2 ** 31:
         raise ValueError(f"{what}: logits {tuple(logits.shape)}")
     if M > 1 and ld < N:
         raise ValueError(f"{what}: rows of the logits overlap (stride {ld} < {N})")
     inv_temp = float(inv_temp)
-    if not 0.0 < inv_temp < math.inf:
-        raise ValueError(f"{what}: inverse temperature {inv_temp} must be positive and finite")
+    if not 0.0 < inv_temp <= 2e38:
+        raise ValueError(f"{what}: inverse temperature {inv_temp} must be positive and at most 2e38")
     return code, M, N, logits.data_ptr(), max(ld, N), inv_temp
 
 

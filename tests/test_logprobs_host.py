@@ -69,6 +69,28 @@ def test_workspace_sizes():
     assert lib.rf_logprobs_workspace(0, 1, 2 ** 31 - 17, 256) >= (2 ** 31 // 32768) * (16 + 8 * 256)
 
 
+def test_sizes_past_a_launch_are_refused():
+    """Column numbers fit 32 bits with a workgroup's reach past the row's end, a launch has at most 2^32 - 1
+    threads, and the plan of very many rows is made in 64 bits."""
+    lib = _lib.load()
+    top = 2 ** 31 - 1
+    assert "shape" in err(fwd(N=top - 2 ** 16 + 1, ld=top))
+    assert "too many" in err(fwd(M=top, N=5, ld=5))
+    assert "too many" in err(fwd(M=2 ** 22, N=70, ld=70, k=65, tv=A, ti=A))
+    assert "too many" in err(lib.rf_token_logprobs_bwd(1, 2 ** 24, 50, A, 50, 1.0, A, A, 1, -100, A, None, None, A, 50,
+                                                       None))
+    assert lib.rf_logprobs_workspace(0, top, 50, 5) == 0
+    assert lib.rf_logprobs_workspace(0, top - 100, 100000, 0) > 0
+    assert "too many" in err(lib.rf_mxfp4_quantize(0, 2 ** 26, 512, A, 512, 1e-8, A, A, None, None))
+    assert "too many" in err(lib.rf_mxfp4_dequantize(0, 2 ** 28, 512, A, A, A, 512, None))
+    assert "too many" in err(lib.rf_mxfp4_gemm(0, top, 1 << 24, 32, A, A, A, A, None, None, None, 1.0, A, 1 << 24,
+                                               None))
+
+
+def test_inverse_temperatures_whose_exponent_overflows_are_refused():
+    assert "temperature" in err(fwd(it=2.5e38))  # times log2(e) it is inf, and 0 * inf no number
+
+
 def test_mxfp4_refusals():
     lib = _lib.load()
     assert "dtype" in err(lib.rf_mxfp4_quantize(3, 1, 32, A, 32, 1e-8, A, A, None, None))
