@@ -359,7 +359,9 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
   }
   // a lane of the fragments reads the words of its four rows i at once
   const int srow = (wave & 1) * 64 + (isw ? Map::wrow(lane & 3, lane >> 2) : (lane & 3) * 16 + (lane >> 2));
-  const int so = srow * KB;
+  // (the second word's 4 bytes are part of the lane's offset: with the scalar offset past the end of an empty
+  //  buffer the range check would be on a number below 0)
+  const int so[2] = {srow * KB, srow * KB + 4};
   const uint8_t* sbase = nullptr;
   int rows = 0;
   __amdgpu_buffer_rsrc_t rc, rs;
@@ -378,8 +380,8 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
           rc, (__attribute__((address_space(3))) void*)(dst + (wave * 8 + p) * 1024), 16, vo[p], kt * 128, 0, 0);
     else if (DW)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rs, (__attribute__((address_space(3))) void*)(dst + MX_CODES + (p - 8) * 1024 + wave * 256), 4, so,
-          8 * kt + 4 * (p - 8), 0, 0);
+          rs, (__attribute__((address_space(3))) void*)(dst + MX_CODES + (p - 8) * 1024 + wave * 256), 4, so[(p - 8) & 1],
+          8 * kt, 0, 0);
   };
   uint32_t pend[2] = {0, 0};  // !DW: this thread's row's scales of the stage on its way
   auto scale_bytes = [&](int kt) {
@@ -389,7 +391,7 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int at = 8 * kt + 4 * d + i;
-        pend[d] |= (uint32_t)(srow < rows && at < KB ? sbase[so + at] : 127) << (8 * i);
+        pend[d] |= (uint32_t)(srow < rows && at < KB ? sbase[so[0] + at] : 127) << (8 * i);
       }
     }
   };
