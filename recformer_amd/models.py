@@ -802,18 +802,27 @@ class RecformerForSeqRec(nn.Module):
     def item_logprobs(self, pooler_output, items=None, k: int = 0, seen=None, want_entropy: bool = False):
         """What the model answers for pooled vectors (B, d), as probabilities over the catalog: log probabilities
         of the given items ((B,) or (B, C) ids) and the k best items under softmax(cos / temp)
-        (ops.token_logprobs). seen: (B, S) item ids to leave out of it (a user's history; -1: none)."""
+        (ops.token_logprobs). seen: (B, S) item ids to leave out of it (a user's history; ids outside the catalog,
+        as -1, leave out nothing)."""
         scores = self.similarity_score(pooler_output)
         if seen is not None:
-            # amin: a slot of -1 leaves column 0 as it is, whatever another slot says of it
-            mask = torch.full(seen.shape, float("-inf"), device=scores.device).masked_fill_(seen < 0, float("inf"))
-            scores = scores.scatter_reduce(1, seen.clamp_min(0), mask, "amin")
+            B, N = scores.shape
+            if seen.dim() != 2 or seen.shape[0] != B:
+                raise ValueError(f"item_logprobs: seen {tuple(seen.shape)} for {B} users: (B, S)")
+            # amin: a slot that leaves out nothing leaves its column as it is, whatever another slot says of it
+            none = (seen < 0) | (seen >= N)
+            mask = torch.full(seen.shape, float("-inf"), device=scores.device).masked_fill_(none, float("inf"))
+            scores = scores.scatter_reduce(1, seen.to(torch.int64).clamp(0, N - 1), mask, "amin")
         return ops.token_logprobs(scores, items, k=k, want_entropy=want_entropy)
 
     def distill_loss(self, teacher_logits, teacher_ids, distill_temp: float = 1.0, **batch):
         """Loss of the batch's catalog scores against a teacher's best items (train.topk_distill_train):
-        teacher_ids (B, K) with their logits or log probabilities (as a teacher's item_logprobs gives them)."""
+        teacher_ids (B, K) with their logits or log probabilities (as a teacher's item_logprobs gives them). The
+        batch holds no labels and no candidates: both take the place of the catalog's scores."""
         from . import train
+        for name in ("labels", "candidates"):
+            if batch.get(name) is not None:
+                raise ValueError(f"distill_loss: {name} in the batch")
         return train.topk_distill_train(self(**batch), teacher_logits, teacher_ids, distill_temp)
 
     def forward(self, input_ids=None, attention_mask=None, global_attention_mask=None, head_mask=None,

@@ -41,6 +41,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import dropout, ops
 
@@ -513,6 +514,13 @@ def cross_entropy_train(logits: torch.Tensor, labels: torch.Tensor, ignore_index
     return _CrossEntropy.apply(logits, labels.reshape(-1).to(torch.int64).contiguous(), ignore_index)
 
 
+def _differentiable_once(backward):
+    """A backward that is refused a second derivative, at the price of a wrapper only where one could be asked for
+    (create_graph)."""
+    guarded = once_differentiable(backward)
+    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     """Log probabilities of given entries and the entropy of softmax(logits * inv_temp), one pass over the
     logits forward (rf_token_logprobs_fwd) and one backward (rf_token_logprobs_bwd, which recomputes the
@@ -528,6 +536,7 @@ class _TokenLogprobs(torch.autograd.Function):
         return r.logp, r.entropy
 
     @staticmethod
+    @_differentiable_once
     def backward(ctx, g_logp, g_entropy):
         if not ctx.needs_input_grad[0] or (g_logp is None and g_entropy is None):
             return None, None, None, None
@@ -546,17 +555,18 @@ class _TopkDistill(torch.autograd.Function):
         val, ids = ops._teacher("topk_distill_train", logits, teacher_logits, teacher_ids)
         _, stats, loss, coef = ops._distill(rows, logits, val, ids, temp * temp)
         ctx.save_for_backward(logits, val, ids, stats, coef)
-        ctx.rows = rows
+        ctx.inv_temp = rows[-1]
         return loss
 
     @staticmethod
+    @_differentiable_once
     def backward(ctx, g):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
         logits, val, ids, stats, coef = ctx.saved_tensors
-        code, M, N, _, ld, inv_temp = ctx.rows
-        return (ops._distill_grad((code, M, N, logits.data_ptr(), ld, inv_temp), logits, stats, val, ids, g, coef),
-                None, None, None)
+        # checked again: hooks on saved tensors may give back rows of another stride
+        rows = ops._logit_rows("topk_distill_train", logits, ctx.inv_temp)
+        return ops._distill_grad(rows, logits, stats, val, ids, g, coef), None, None, None
 
 
 def token_logprobs_train(logits: torch.Tensor, tokens: torch.Tensor, inv_temp: float = 1.0, ignore_index: int = -100):

@@ -466,3 +466,70 @@ def test_model_answers_and_learns_from_a_teacher(dev):
     logits = lm.lm_logits(hidden)
     close_logp(r.logp, torch.where(words < 0, 0.0, ref_softmax(logits, 1.0)[0].gather(1, words.clamp_min(0)[:, None])[:, 0]))
     check_top(logits, r, 3, 1.0)
+
+
+@pytest.mark.parametrize("N,pad", [(50, 6), (4100, 3)])
+def test_gradients_through_saved_tensor_hooks(dev, N, pad):
+    """Hooks that keep saved tensors elsewhere (offloading) may hand the logits back with other strides: the
+    gradient is the same."""
+    buf = torch.full((5, N + pad), float("nan"), device=dev)
+    buf[:, :N] = logits_of(dev, torch.float32, 5, N, 3)
+    ids = torch.randint(0, N, (5, 4), device=dev)
+    tl = torch.randn(5, 4, device=dev)
+
+    def grads(x):
+        leaf = x.detach().requires_grad_()
+        logp, h = train.token_logprobs_train(leaf, ids)
+        loss = train.topk_distill_train(leaf, tl, ids, 2.0)
+        return leaf, loss + logp.sum() + h.sum()
+
+    leaf, out = grads(buf[:, :N])
+    want, = torch.autograd.grad(out, leaf)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t):
+        leaf, out = grads(buf[:, :N])
+    got, = torch.autograd.grad(out, leaf)
+    assert torch.equal(got, want)
+
+
+def test_second_derivatives_are_refused(dev):
+    ids = torch.tensor([[1, 2], [3, 4]], device=dev)
+    for fn in (lambda x: train.token_logprobs_train(x, ids)[0].sum(),
+               lambda x: train.token_logprobs_train(x, ids)[1].sum(),
+               lambda x: train.topk_distill_train(x, torch.randn(2, 2, device=dev), ids)):
+        leaf = logits_of(dev, torch.float32, 2, 50, 1).requires_grad_()
+        d, = torch.autograd.grad(fn(leaf), leaf, create_graph=True)
+        assert bool(torch.isfinite(d).all())
+        with pytest.raises(RuntimeError):
+            d.square().sum().backward()
+
+
+def test_history_ids_outside_the_catalog_leave_out_nothing(dev):
+    """A padding id of N, or an id of another catalog, in the history; int32 ids; no slot at all; a history of
+    other users; and batches that would not give the catalog's scores are refused."""
+    from recformer_amd.hashinit import hash_tensor
+    from recformer_amd.models import RecformerForSeqRec
+    from recformer_amd.synth import C1
+    from tests.common import hashed_model
+    m = hashed_model(dict(C1, item_num=70), 1, RecformerForSeqRec)
+    m.init_item_embedding(hash_tensor("items", (70, C1["hidden_size"]), "weight", std=1.0))
+    m = m.to(dev)
+    z = torch.randn(2, C1["hidden_size"], device=dev)
+    want = m.item_logprobs(z, k=70, seen=torch.tensor([[69, 4], [0, -1]], device=dev))
+    got = m.item_logprobs(z, k=70, seen=torch.tensor([[69, 4, 70, 2 ** 30], [70, 0, -5, 71]], device=dev, dtype=torch.int32))
+    assert torch.equal(want.top_ids, got.top_ids) and torch.equal(want.top_logp, got.top_logp)
+    assert bool((got.top_logp[:, -1] == -INF).all()) and bool(torch.isfinite(got.top_logp[:, :68]).all())
+    plain = m.item_logprobs(z, k=5)
+    none = m.item_logprobs(z, k=5, seen=torch.zeros(2, 0, dtype=torch.long, device=dev))
+    # the scores' rows are 72 columns apart and the masked copy's 70, so the copy's second row is cut into other
+    # chunks and its sum is taken in another order: each is within close_logp's bound of the exact value, and
+    # the two of each other within twice that
+    assert torch.equal(plain.top_ids, none.top_ids)
+    d = (plain.top_logp.double() - none.top_logp.double()).abs()
+    assert bool((d <= 2 * (160 * U + 4 * U * plain.top_logp.double().abs())).all())
+    with pytest.raises(ValueError):
+        m.item_logprobs(z, k=5, seen=torch.zeros(3, 1, dtype=torch.long, device=dev))
+    with pytest.raises(ValueError):
+        m.distill_loss(torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.long), labels=torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError):
+        m.distill_loss(torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.long),
+                       candidates=torch.zeros(2, 3, dtype=torch.long))
