@@ -702,27 +702,35 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
 // ---- host --------------------------------------------------------------------------------------
 static int lp_vec(int dtype) { return dtype == RF_F32 ? 4 : 8; }
 
-// Slices per row and chunks per slice. A slice is at most what a 1024-thread workgroup holds. Fewer rows
-// than two workgroups a CU are cut further, down to LP_MIN_CHUNKS chunks (8 KB, two chunks a thread of a
-// 256-thread workgroup), as long as the lists that the join reads stay within 16 entries a thread.
-constexpr int LP_CUS = 256, LP_MIN_CHUNKS = 512;
+// Slices per row and chunks per slice. A slice is at most what a 1024-thread workgroup holds. A row that one
+// workgroup holds is not cut, however few the rows: the join's launch costs more than the shorter slices give (uncut
+// against 8 KB slices: 64 x 10000 fp32 top 50 8.7 and 13.6 us, 300 x 50265 top 20 15.0 and 21.7; the other way
+// only for a row or two without alternatives, 1 x 50265 7.5 and 6.5). Rows that are joined anyway, and fewer than
+// two workgroups a CU, are cut further, down to LP_MIN_CHUNKS chunks (1 x 70000: 6.4 us, 9.1 uncut, 4 x 1M bf16
+// 7.3 and 11.0), as long as the join reads at most LP_JOIN entries a row (1 x 1M top 256 in 64 slices instead of
+// 31: 76 and 62 us, 4 x 1M top 50 in 128 instead of 31: 20.0 and 18.5).
+constexpr int LP_CUS = 256, LP_MIN_CHUNKS = 512, LP_JOIN = 4096;
 static void lp_plan(int dtype, int M, int N, int k, int* S, int* cps) {
   const int V = lp_vec(dtype);
   const int64_t nch = ((int64_t)N + 2 * V - 2) / V;  // of a row that starts anywhere in a chunk
   int64_t s = (nch + 1024 * LP_R - 1) / (1024 * LP_R);
-  const int64_t want = std::min({(2 * LP_CUS + (int64_t)M - 1) / M, nch / LP_MIN_CHUNKS,
-                                 (int64_t)16384 / std::max(k, 16)});
-  s = std::max(s, want);
-  s = std::max<int64_t>(s, 1);
+  if (s > 1) {
+    const int64_t want = std::min({(2 * LP_CUS + (int64_t)M - 1) / M, nch / LP_MIN_CHUNKS,
+                                   (int64_t)LP_JOIN / std::max(k, 1)});
+    s = std::max(s, want);
+  }
   *cps = (int)((nch + s - 1) / s);
   *S = (int)((nch + *cps - 1) / *cps);
 }
 
-// threads of a workgroup: one wave a row where rows are short and fill the card, 1024 where a slice needs them
-// or many alternatives want many groups, 256 otherwise
+// Threads of a workgroup. One wave a row where it has a chunk a thread, or up to LP_R where rows fill the card (64
+// against 256 threads, bf16 top 10: 8192 x 500 13.3 and 28.2 us, 8192 x 4000 23.7 and 30.7, 512 x 500 6.0 and
+// 7.1; but 1024 x 4000 9.2 and 8.3, 64 x 2000 fp32 8.6 and 6.4); a wave's 64 maxima bound up to 32
+// alternatives well. 256 threads (against 1024: 2048 x 10000 top 20 16 and 34 us, top 128 29 and 54) up to 128
+// alternatives; for more their 256 maxima bound badly (2048 x 10000 top 224: 91 and 80 us, 64 x 16000 55 and 17).
 static int lp_threads(const LpArgs& a) {
-  if (a.cps <= 64 * LP_R && a.S == 1 && a.M >= 2048 && a.k <= 16) return 64;
-  return a.cps <= 256 * LP_R && a.k <= 64 ? 256 : 1024;
+  if (a.S == 1 && a.k <= 32 && (a.cps <= 64 || (a.cps <= 64 * LP_R && a.M >= 2048))) return 64;
+  return a.cps <= 256 * LP_R && a.k <= 128 ? 256 : 1024;
 }
 
 template <typename T, bool ENT, bool TOP, bool TEACH>
@@ -734,6 +742,8 @@ static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
   else if (tpb == 256) k_logprobs<T, 256, ENT, TOP, TEACH><<<grid, 256, 0, st>>>(a, p);
   else k_logprobs<T, 1024, ENT, TOP, TEACH><<<grid, 1024, 0, st>>>(a, p);
   if (a.S > 1) {
+    // 256 threads for short lists (1 x 50265 in 12 slices, top 5: 10.2 and 11.0 us), 1024 for long ones (4 x 1M, 128
+    // lists of 50: 26.7 and 19.9)
     if (!TOP || (a.S * a.k <= 2048 && a.k <= 64)) k_logprobs_join<T, 256, TOP, TEACH><<<a.M, 256, 0, st>>>(a, p);
     else k_logprobs_join<T, 1024, TOP, TEACH><<<a.M, 1024, 0, st>>>(a, p);
   }

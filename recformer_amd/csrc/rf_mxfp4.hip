@@ -242,7 +242,8 @@ struct MxVec {
 // A wave's 64 x 64 results to rows mw.., columns nw..: acc[i][j] holds columns MxMap::wrow(i, 4 g ..) of row
 // j 16 + r. A lane holds 16 bytes of a row at a time, and the same 64 bytes further on: lanes of rows r and r + 1
 // (r even) trade, so that the even lane holds the first piece of both rows and the odd lane the second, and a
-// store writes whole 128-byte lines (64-byte halves took 893 instead of 779 us at 4096 x 125000 fp32).
+// store writes whole 128-byte lines (non-temporal 64-byte halves took 1625 instead of 1229 us at 4096 x 125000 fp32 with
+// rows off the lines; with rows on lines it takes 515).
 // EDGE: element by element, those outside of C at an offset that the buffer store drops.
 template <typename T, bool EDGE>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, int64_t mw, int64_t nw, int r, int g,
@@ -501,7 +502,9 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
 }
 
 // Up to 16 MT rows of A: W is read once from memory straight into the fragments, a wave per 16 NT of its rows,
-// U steps of K in flight; the A rows come from the caches. Bound by the read of W. DW: a row's four scales of
+// U steps of K in flight; the A rows come from the caches. Bound by the read of W for few rows (1 x 1M x 768 88 us,
+// 4.7 TB/s; 1 x 100000 x 4096 41 us, 5.3 TB/s), by the A fragments' way through the caches for many (64 x 1M x 768
+// 231 us, 2.9 TB/s with the result). DW: a row's four scales of
 // a step are one word; the four lanes of a row load the words of four steps and trade them (a byte a lane and
 // step took 66 instead of 41 us at 1 x 100000 x 4096).
 template <typename T, int MT, int NT, bool DW>
@@ -606,18 +609,31 @@ static int lane_shift(int K) {  // lanes a row: enough for its eights, at least 
   return sh;
 }
 
-template <typename T, int MT, bool DW>
+template <typename T, int NT, bool DW>
 static void launch_skinny(const MxArgs& a, hipStream_t st) {
-  // four row tiles a wave share the A fragments; one where that would leave CUs without waves
-  if (a.N >= 64 * 4 * 512) k_mxfp4_skinny<T, MT, 4, DW><<<(unsigned)((a.N + 255) / 256), 256, 0, st>>>(a);
-  else k_mxfp4_skinny<T, MT, 1, DW><<<(unsigned)((a.N + 63) / 64), 256, 0, st>>>(a);
+  const unsigned grid = (unsigned)((a.N + 64 * NT - 1) / (64 * NT));
+  if (a.M <= 16) k_mxfp4_skinny<T, 1, NT, DW><<<grid, 256, 0, st>>>(a);
+  else if (a.M <= 32) k_mxfp4_skinny<T, 2, NT, DW><<<grid, 256, 0, st>>>(a);
+  else k_mxfp4_skinny<T, 4, NT, DW><<<grid, 256, 0, st>>>(a);
 }
 
+// Up to 64 rows a wave streams one tile of W's rows, or four that share the A fragments; the tile kernel shares W's
+// lines through LDS as well and hides a long K better. Four: for more columns than two workgroups of one tile a CU,
+// while K is short. One: for fewer (for 17 to 64 rows while its workgroups are one a CU), and for up to 4 rows,
+// whose fragments cost little.
+// us for one tile / four / tile kernel, fp32 results, the table read again and again:
+//   K = 512:   1 x 400k 18.6 20.4 29.4; 16 x 400k 30.8 27.2 39.7; 64 x 50k 15.7 13.1 14.8; 64 x 16k 6.1 11.3 8.4
+//   K = 1024:  1 x 400k 35.9 39.4 41.9; 32 x 400k 88.8 65.4 66.7; 64 x 400k 164 105 105;   64 x 16k 9.0 16.1 9.9
+//   K = 1536: 16 x 400k 90.9 84.9 85.0; 32 x 400k 130 107 102;    64 x 400k 228 144 135;   64 x 16k 11.0 19.3 11.2
+//   K = 4096:  1 x 400k 158 192 181;    16 x 400k 255 225 208;    32 x 16k 16.3 31.5 20.9; 64 x 16k 25.6 42.5 23.1
+// From HBM, 1 x 1M x 768: 93.6 and 87.5 us (4.7 TB/s) for one and four.
 template <typename T, bool DW>
 static void launch_gemm(const MxArgs& a, hipStream_t st) {
-  if (a.M <= 16) return launch_skinny<T, 1, DW>(a, st);
-  if (a.M <= 32) return launch_skinny<T, 2, DW>(a, st);
-  if (a.M <= 64) return launch_skinny<T, 4, DW>(a, st);
+  constexpr int cols = 64 * 256;  // of one workgroup a CU, a tile a wave
+  const bool four = a.N > 2 * cols && a.KB <= (a.M <= 16 ? 48 : 32);
+  const bool one = a.M <= 4 || (a.N <= (a.M <= 16 ? 2 : 1) * cols && (a.M <= 32 || a.KB <= 48));
+  if (a.M <= 64 && four) return launch_skinny<T, 4, DW>(a, st);
+  if (a.M <= 64 && one) return launch_skinny<T, 1, DW>(a, st);
   constexpr int lds = 2 * MX_STAGE;
   (void)hipFuncSetAttribute((const void*)k_mxfp4_gemm<T, DW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   k_mxfp4_gemm<T, DW><<<(unsigned)std::min(a.nTm * a.nTn, MX_WGS), 256, lds, st>>>(a);
@@ -700,7 +716,8 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
   a.nTn = (N + MX_T - 1) / MX_T;
   // row tiles whose codes fill half of an XCD's 4 MB of L2
   a.gm = (int)std::max<int64_t>(1, std::min<int64_t>(a.nTm, (2 << 20) / ((int64_t)MX_T * a.KB * 16)));
-  a.gn = 4;  // column tiles side by side: 1 to 32 took within 3% of each other
+  // column tiles side by side (1, 4, 8: 428, 413, 416 us at 4096 x 125000 x 768 fp32; 8192^3 373, 379, 384)
+  a.gn = 4;
   RF_REQUIRE((int64_t)a.nTm * a.nTn < 0x7FFFFFFF - MX_WGS, "rf_mxfp4_gemm: too many tiles");
   hipStream_t st = as_stream(stream);
   const bool dw = a.KB % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.as) | reinterpret_cast<uintptr_t>(a.ws)) & 3) == 0;

@@ -166,6 +166,14 @@ def test_product(dev, out, M, N, K):
     close(ops.mxfp4_gemm(a, w, bias, out, ra, rw, 0.05), want * f + bias.double(), size * f + bias.double().abs())
 
 
+@pytest.mark.parametrize("M,N,K", [(2, 33000, 64), (5, 32769, 256), (16, 33001, 160), (16, 32770, 1600), (20, 20000, 96),
+                                   (32, 33003, 128), (17, 40007, 33), (64, 32800, 512), (40, 33333, 200),
+                                   (64, 33000, 1056), (33, 32768, 64), (50, 700, 1568)])
+def test_product_of_few_rows_and_many_columns(dev, M, N, K):
+    """Few rows against long tables, on both sides of where the work is laid out differently."""
+    test_product(dev, torch.float32, M, N, K)
+
+
 def test_product_quantises_rows_on_the_way(dev):
     for dt in DTYPES:
         x = rows_of(dev, dt, 70, 200, 5, "offset")
