@@ -206,11 +206,76 @@ __device__ __forceinline__ void find_tau(SelectLds<TPB>& s, int lane, int k) {
   if (lane == 0) s.tau = tau;
 }
 
+// The exact search: collects into s.cand the min(k, n) best of src.all's n entries by the digits (8 bits from the top)
+// of the last one taken; stops as soon as a digit's whole bin is taken. It is rare, and a function of its own so
+// that its registers do not crowd out the short way's.
+template <int TPB, typename Src>
+__device__ __attribute__((noinline)) int collect_exact(const Src src, int k, int64_t n, SelectLds<TPB>* sel) {
+  SelectLds<TPB>& s = *sel;
+  const int t = threadIdx.x;
+  const int kk = (int)(n < k ? n : k);
+  uint64_t prefix = 0;
+  int rem = kk, shift = 64;
+  while (true) {
+    __syncthreads();
+    for (int i = t; i < 256; i += TPB) s.key[i] = 0;
+    __syncthreads();
+    src.all([&](uint64_t e) {
+      if (shift != 64 && (e >> shift) != prefix) return;
+      const int d = (int)(e >> (shift - 8)) & 255;
+      const uint64_t here = __ballot(1);
+      if (__ballot(d == __builtin_amdgcn_readfirstlane(d)) == here) {  // adds to one address would go one by one
+        if ((t & 63) == __builtin_ctzll(here)) atomicAdd(&s.key[d], (uint32_t)__popcll(here));
+      } else {
+        atomicAdd(&s.key[d], 1u);
+      }
+    });
+    __syncthreads();
+    if (t < 64) {  // four digits a lane, the highest first
+      int h[4], sum = 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sum += h[x] = (int)s.key[255 - 4 * t - x];
+      int above = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(above, o, 64);
+        if (t >= o) above += v;
+      }
+      above -= sum;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (above < rem && above + h[x] >= rem) {  // one lane's, once
+          s.prefix = prefix << 8 | (uint64_t)(255 - 4 * t - x);
+          s.rem = rem - above;
+          s.done = h[x] == rem - above;
+        }
+        above += h[x];
+      }
+    }
+    __syncthreads();
+    prefix = s.prefix;
+    rem = s.rem;
+    shift -= 8;
+    if (s.done || shift == 0) break;
+  }
+  const uint64_t least = prefix << shift;
+  __syncthreads();
+  if (t == 0) s.count = 0;
+  __syncthreads();
+  src.all([&](uint64_t e) {
+    if (e < least) return;
+    const int at = atomicAdd(&s.count, 1);
+    if (at < SelectLds<TPB>::CAP) s.cand[at] = e;
+  });
+  __syncthreads();
+  return min(s.count, SelectLds<TPB>::CAP);
+}
+
+
 // Collects into s.cand what passes s.tau, at least min(k, n) entries and among them the k best, and returns how
 // many. src.each(tau, f) calls f(entry) for every entry of the calling thread whose key is >= tau,
-// src.again(f) for all its entries; nan: some value is NaN (the float compares of src.each would miss it).
-// Where more than CAP entries pass (many equal values, or the best all in few threads) an exact search over
-// the 64-bit entries by 8-bit digits follows; its threshold lets exactly min(k, n) through.
+// src.again().all(f) for all its entries; nan: some value is NaN (the float compares of src.each would miss it).
+// Where more than CAP entries pass (many equal values, or the best all in few threads) the exact search follows.
 template <int TPB, typename Src>
 __device__ __forceinline__ int collect(const Src& src, bool nan, int k, int64_t n, SelectLds<TPB>& s) {
   const int t = threadIdx.x;
@@ -224,56 +289,30 @@ __device__ __forceinline__ int collect(const Src& src, bool nan, int k, int64_t 
     const int c = s.count;
     if (c <= SelectLds<TPB>::CAP) return c;
   }
-  // exact: the digits of the k-th largest entry from the top; stops as soon as a digit's whole bin is taken
-  const int kk = (int)(n < k ? n : k);
-  uint64_t prefix = 0;
-  int rem = kk, shift = 64;
-  while (true) {
-    __syncthreads();
-    for (int i = t; i < 256; i += TPB) s.key[i] = 0;
-    __syncthreads();
-    src.again([&](uint64_t e) {
-      if (shift == 64 || (e >> shift) == prefix) atomicAdd(&s.key[(e >> (shift - 8)) & 255], 1u);
-    });
-    __syncthreads();
-    if (t == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + (int)s.key[d] < rem) above += s.key[d--];
-      s.prefix = prefix << 8 | (uint64_t)d;
-      s.rem = rem - above;
-      s.done = (int)s.key[d] == rem - above;
-    }
-    __syncthreads();
-    prefix = s.prefix;
-    rem = s.rem;
-    shift -= 8;
-    if (s.done || shift == 0) break;
-  }
-  const uint64_t least = prefix << shift;
-  __syncthreads();
-  if (t == 0) s.count = 0;
-  __syncthreads();
-  src.again([&](uint64_t e) {
-    if (e >= least) take(e);
-  });
-  __syncthreads();
-  return min(s.count, SelectLds<TPB>::CAP);
+  return collect_exact<TPB>(src.again(), k, n, &s);
 }
 
 // f(rank, entry) for the candidates in list order: entries are all different, so an entry's rank is the
-// number of larger ones (counted by one lane each: several lanes an entry took 4% longer at 4915 x 50265)
-template <int TPB, typename F>
-__device__ __forceinline__ void rank_candidates(const SelectLds<TPB>& s, int c, int k, F f) {
-  for (int i = threadIdx.x; i < c; i += TPB) {
+// number of larger ones. Counted by one lane each (several lanes an entry took 4% longer at 4915 x 50265 top 20),
+// by two where there are many.
+template <int TPB, int L, typename F>
+__device__ __forceinline__ void rank_by(const SelectLds<TPB>& s, int c, int k, F f) {  // L lanes an entry
+  for (int i = threadIdx.x / L; i < c; i += TPB / L) {
     const uint64_t e = s.cand[i];
-    int r = 0, j = 0;
-    for (; j + 4 <= c; j += 4) {  // reads of four together: their latencies overlap
+    int r = 0, j = 4 * (threadIdx.x % L);
+    for (; j + 4 <= c; j += 4 * L) {  // reads of four together: their latencies overlap
       const uint64_t a0 = s.cand[j], a1 = s.cand[j + 1], a2 = s.cand[j + 2], a3 = s.cand[j + 3];
       r += (a0 > e) + (a1 > e) + (a2 > e) + (a3 > e);
     }
     for (; j < c; ++j) r += s.cand[j] > e;
-    if (r < k) f(r, e);
+    if (L == 2) r += __builtin_amdgcn_mov_dpp(r, 0xB1, 0xF, 0xF, true);  // the neighbour's
+    if (r < k && (L == 1 || !(threadIdx.x & 1))) f(r, e);
   }
+}
+template <int TPB, typename F>
+__device__ __forceinline__ void rank_candidates(const SelectLds<TPB>& s, int c, int k, F f) {
+  if (TPB == 1024 && c > 128) rank_by<TPB, 2>(s, c, k, f);
+  else rank_by<TPB, 1>(s, c, k, f);
 }
 
 // ---- what a finished row gives -----------------------------------------------------------------
@@ -403,12 +442,17 @@ struct RowSrc {
       }
     }
   }
-  template <typename F>
-  __device__ __forceinline__ void again(F f) const {
+  struct Again {
+    const T* x;
+    int64_t c0, c1;
+    template <typename F>
+    __device__ __forceinline__ void all(F f) const {
+      for (int64_t c = c0 + threadIdx.x; c < c1; c += TPB) f(entry_of(to_f32(x[c]), (uint32_t)c));
+    }
+  };
+  __device__ __forceinline__ Again again() const {
     constexpr int V = Row<T>::V;
-    const int64_t c1 = min((int64_t)(j0 + jn) * V - off, (int64_t)N);
-    for (int64_t c = max((int64_t)j0 * V - off, (int64_t)0) + threadIdx.x; c < c1; c += TPB)
-      f(entry_of(to_f32(x[c]), (uint32_t)c));
+    return {x, max((int64_t)j0 * V - off, (int64_t)0), min((int64_t)(j0 + jn) * V - off, (int64_t)N)};
   }
 };
 
@@ -510,16 +554,19 @@ __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a,
 template <int TPB>
 struct ListSrc {
   const uint64_t* ent;
-  int n;
+  uint32_t S, k;
+  // the lists' first entries before their second ones: a thread's entries are of different ranks, so the threads'
+  // maxima are the best of all lists (in the lists' own order the bound let 2048 of 16 lists of 256 through)
   template <typename F>
   __device__ __forceinline__ void each(uint32_t tau, F f) const {
-    for (int i = threadIdx.x; i < n; i += TPB) {
-      const uint64_t e = ent[i];
+    for (uint32_t i = threadIdx.x; i < S * k; i += TPB) {
+      const uint64_t e = ent[i % S * k + i / S];
       if (e != 0 && (uint32_t)(e >> 32) >= tau) f(e);
     }
   }
+  __device__ __forceinline__ ListSrc again() const { return *this; }
   template <typename F>
-  __device__ __forceinline__ void again(F f) const { each(0u, f); }
+  __device__ __forceinline__ void all(F f) const { each(0u, f); }
 };
 
 template <typename T, int TPB, bool TOP, bool TEACH>
@@ -548,9 +595,9 @@ __global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __rest
   block_sum2<TPB>(s, h, red);
   finish_row<TPB, TEACH>(a, r, x, m, s, h, own, red);
   if (TOP) {
-    const ListSrc<TPB> src{a.pent + (int64_t)r * a.S * a.k, a.S * a.k};
+    const ListSrc<TPB> src{a.pent + (int64_t)r * a.S * a.k, (uint32_t)a.S, (uint32_t)a.k};
     uint64_t best = 0;
-    src.again([&](uint64_t e) { best = max(best, e); });
+    src.all([&](uint64_t e) { best = max(best, e); });
     sel.key[t] = (uint32_t)(best >> 32);
     if (t == 0) sel.count = 0;
     __syncthreads();
