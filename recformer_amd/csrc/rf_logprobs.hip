@@ -371,21 +371,30 @@ __device__ __forceinline__ void finish_row(const LpArgs& a, int r, const T* __re
   };
   float tm = 0.f, trs = 0.f;
   if constexpr (TEACH) {
-    float mx = LP_NINF;
-    each([&](int, const Listed<TEACH>& l) {
-      if (l.id != -1) mx = fmaxf(mx, l.t);
-    });
-    tm = block_max<TPB>(mx, red);
-    if (tm == LP_NINF) tm = 0.f;
+    auto top = [&](float mx, const Listed<TEACH>& l) { return l.id != -1 ? fmaxf(mx, l.t) : mx; };
     float ts = 0.f, cross = 0.f;
-    each([&](int, const Listed<TEACH>& l) {
+    auto add = [&](const Listed<TEACH>& l) {
       if (l.id == -1) return;
       const float tz = (l.t - tm) * a.it;
       const float e = __builtin_amdgcn_exp2f(tz * LP_LOG2E);
       ts += e;
       if (e != 0.f) cross += e * (tz - logp(l.x));  // a teacher logit of -inf teaches nothing, whatever the student says
-    });
-    block_sum2<TPB>(ts, cross, red);
+    };
+    if (a.nids <= 64) {  // the first wave's entries: no barriers
+      if (t >= 64) return;
+      tm = wave_max(top(LP_NINF, own));
+      if (tm == LP_NINF) tm = 0.f;
+      add(own);
+      ts = wave_sum(ts);
+      cross = wave_sum(cross);
+    } else {
+      float mx = LP_NINF;
+      each([&](int, const Listed<TEACH>& l) { mx = top(mx, l); });
+      tm = block_max<TPB>(mx, red);
+      if (tm == LP_NINF) tm = 0.f;
+      each([&](int, const Listed<TEACH>& l) { add(l); });
+      block_sum2<TPB>(ts, cross, red);
+    }
     trs = ts == 0.f ? 0.f : 1.f / ts;
     // sum q (tz - ln ts - logp) with q = e / ts
     if (t == 0) a.logp[r] = ts == 0.f ? 0.f : cross * trs - __builtin_amdgcn_logf(ts) * LP_LN2;
