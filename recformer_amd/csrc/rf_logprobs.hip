@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(1024) k_rows_mean(int M, const float* __restri
 }
 
 // ---- gradients ---------------------------------------------------------------------------------
-constexpr int LB_R = 4, LB_TPB = 256;
+constexpr int LB_R = 4;
 
 struct LpBwdArgs {
   int M, N, S, cps;
@@ -657,13 +657,14 @@ struct LpBwdArgs {
 // One slice of a row: read, e^t / s, write. The listed entries are then written again by one thread each
 // (after a barrier; the first of equal ids adds all their weights in list order), so nothing is added
 // atomically.
-template <typename T, bool ENT>
-__global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* __restrict__ logits,
+template <typename T, int TPB, bool ENT>
+__global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __restrict__ logits,
                                                          T* __restrict__ dlogits) {
   constexpr int V = Row<T>::V;
   __shared__ float red[32];
-  __shared__ int32_t sid[LP_LIST];
-  __shared__ float sw[LP_LIST];
+  constexpr int LIST = TPB == 64 ? 64 : LP_LIST;
+  __shared__ int32_t sid[LIST];
+  __shared__ float sw[LIST];
   const int t = threadIdx.x;
   const int r = blockIdx.x / a.S, sl = blockIdx.x % a.S;
   const T* x = logits + (int64_t)r * a.ld;
@@ -674,7 +675,7 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
   u32x4 raw[LB_R];
 #pragma unroll
   for (int i = 0; i < LB_R; ++i) {
-    const int j = i * LB_TPB + t;
+    const int j = i * TPB + t;
     if (j < jn) raw[i] = load_chunk(x, (j0 + j) * V - off, a.N);
   }
   const float m = a.stats[4 * (int64_t)r], rs = a.stats[4 * (int64_t)r + 1];
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
     const float tm = a.stats[4 * (int64_t)r + 2], trs = a.stats[4 * (int64_t)r + 3];
     const float g = a.g[0] * a.coef[0];
     float bad = 0.f, unused = 0.f;
-    for (int j = t; j < a.nids; j += LB_TPB) {
+    for (int j = t; j < a.nids; j += TPB) {
       const int64_t id = a.ids[(int64_t)r * a.nids + j];
       const float q = id == -1 ? 0.f : __builtin_amdgcn_exp2f((a.tval[(int64_t)r * a.nids + j] - tm) * a.c2) * trs;
       const bool in = id >= 0 && id < a.N;
@@ -693,11 +694,11 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
       sid[j] = in && q != 0.f ? (int32_t)id : -1;
       sw[j] = -g * q;
     }
-    block_sum2<LB_TPB>(bad, unused, red);
+    block_sum2<TPB>(bad, unused, red);
     ca = trs == 0.f ? 0.f : g + bad;
   } else {
     float sum = 0.f, unused = 0.f;
-    for (int j = t; j < a.nids; j += LB_TPB) {
+    for (int j = t; j < a.nids; j += TPB) {
       const int64_t id = a.ids[(int64_t)r * a.nids + j];
       const bool in = id >= 0 && id < a.N;
       const float g = a.g && id != a.ignore ? a.g[(int64_t)r * a.nids + j] : 0.f;
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
       sid[j] = in && id != a.ignore ? (int32_t)id : -1;
       sw[j] = g;
     }
-    block_sum2<LB_TPB>(sum, unused, red);
+    block_sum2<TPB>(sum, unused, red);
     ca = -sum;
     if (ENT) {
       cb = -a.g_ent[r];
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
   };
 #pragma unroll
   for (int i = 0; i < LB_R; ++i) {
-    const int j = i * LB_TPB + t;
+    const int j = i * TPB + t;
     if (j < jn) {
       const int64_t c0 = (int64_t)(j0 + j) * V - off;
       T o[V];
@@ -741,7 +742,7 @@ __global__ void __launch_bounds__(LB_TPB) k_logprobs_bwd(LpBwdArgs a, const T* _
   if (empty) return;
   __syncthreads();
   const int64_t first = (int64_t)j0 * V - off, last = (int64_t)(j0 + jn) * V - off;
-  for (int j = t; j < a.nids; j += LB_TPB) {
+  for (int j = t; j < a.nids; j += TPB) {
     const int32_t id = sid[j];
     if (id < 0 || id < first || id >= last) continue;
     float w = 0.f;
@@ -855,18 +856,25 @@ static int lp_backward(const char* name, int dtype, const LpBwdArgs& in, const v
                  (a.ld - a.ldd) % V == 0,
              "%s: the gradient's rows must be aligned as the logits' rows are", name);
   const int64_t nch = ((int64_t)a.N + 2 * V - 2) / V;
-  a.S = (int)((nch + LB_TPB * LB_R - 1) / (LB_TPB * LB_R));
+  // one wave a row where that holds it (256 threads: 8192 x 500 bf16 with 20 teacher entries 17.7 us instead of 10.9,
+  // 100000 x 100 170 instead of 75)
+  const int tpb = nch <= 64 * LB_R && a.nids <= 64 ? 64 : 256;
+  a.S = (int)((nch + tpb * LB_R - 1) / (tpb * LB_R));
   a.cps = (int)((nch + a.S - 1) / a.S);
-  RF_REQUIRE((int64_t)a.M * a.S * LB_TPB <= 0xFFFFFFFFll, "%s: %d rows of %d slices are too many for a launch", name,
+  RF_REQUIRE((int64_t)a.M * a.S * tpb <= 0xFFFFFFFFll, "%s: %d rows of %d slices are too many for a launch", name,
              a.M, a.S);
   const unsigned grid = (unsigned)((int64_t)a.M * a.S);
-#define LB_T(T)                                                                                        \
-  if (a.g_ent) k_logprobs_bwd<T, true><<<grid, LB_TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits);       \
-  else k_logprobs_bwd<T, false><<<grid, LB_TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits)
+#define LB_K(T, TPB, ENT) k_logprobs_bwd<T, TPB, ENT><<<grid, TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits)
+#define LB_T(T)                                 \
+  if (tpb == 64 && a.g_ent) LB_K(T, 64, true);  \
+  else if (tpb == 64) LB_K(T, 64, false);       \
+  else if (a.g_ent) LB_K(T, 256, true);         \
+  else LB_K(T, 256, false)
   if (dtype == RF_F32) { LB_T(float); }
   else if (dtype == RF_BF16) { LB_T(bf16); }
   else { LB_T(f16); }
 #undef LB_T
+#undef LB_K
   RF_LAUNCH_CHECK(name);
 }
 

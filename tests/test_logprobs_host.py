@@ -77,7 +77,7 @@ def test_sizes_past_a_launch_are_refused():
     assert "shape" in err(fwd(N=top - 2 ** 16 + 1, ld=top))
     assert "too many" in err(fwd(M=top, N=5, ld=5))
     assert "too many" in err(fwd(M=2 ** 22, N=200, ld=200, k=129, tv=A, ti=A))
-    assert "too many" in err(lib.rf_token_logprobs_bwd(1, 2 ** 24, 50, A, 50, 1.0, A, A, 1, -100, A, None, None, A, 50,
+    assert "too many" in err(lib.rf_token_logprobs_bwd(1, 2 ** 26, 50, A, 50, 1.0, A, A, 1, -100, A, None, None, A, 50,
                                                        None))
     assert lib.rf_logprobs_workspace(0, top, 50, 5) == 0
     assert lib.rf_logprobs_workspace(0, top - 100, 100000, 0) > 0
