@@ -30,10 +30,10 @@ __device__ __forceinline__ float quad(float v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* x, int c, int K, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= K) {
+__device__ __forceinline__ void load8(const T* x, int c, int K, float (&v)[8]) {
+  if (c + 8 <= K) {
     T e[8];
-    __builtin_memcpy(e, __builtin_assume_aligned(x + c, 16), sizeof(e));
+    __builtin_memcpy(e, x + c, sizeof(e));  // 16 bytes at any alignment (element by element 100000 x 770 bf16 took 90 us instead of 39)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
   } else {
@@ -43,10 +43,10 @@ __device__ __forceinline__ void load8(const T* x, int c, int K, bool vec, float 
 }
 
 // A row is taken by 2^sh lanes, eight values a lane at a time, four lanes a block. HBM bound (read the
-// row, write 17 bytes a block).
+// row, write 17 bytes a block): 1M x 768 bf16 395 us, 4.9 TB/s, with the norms 432.
 template <typename T>
 __global__ void __launch_bounds__(256) k_mxfp4_quantize(int64_t M, int K, int KB, const T* __restrict__ x, int64_t ldx,
-                                                        int sh, bool vec, float eps, uint8_t* __restrict__ codes,
+                                                        int sh, float eps, uint8_t* __restrict__ codes,
                                                         uint8_t* __restrict__ scales, float* __restrict__ rnorm) {
   const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t row = gid >> sh;
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) k_mxfp4_quantize(int64_t M, int K, int KB
   float sq = 0.f;
   for (int c = 8 * sub; c < KB * 32; c += 8 * L) {
     float v[8];
-    load8(xr, c, K, vec, v);
+    load8(xr, c, K, v);
     float top = 0.f;
     bool bad = false;
 #pragma unroll
@@ -95,7 +95,8 @@ __device__ __forceinline__ float scale_value(int s) {  // 2^(s - 127); 255: NaN
 
 // Eights of values, flat over the rows (G = ceil(K / 8) a row), two a thread 64 apart so that a wave's loads and
 // stores are contiguous. HBM bound; the stores are non-temporal (1M x 768 to bf16: 318 us, 6.1 TB/s; 538 us
-// through the caches).
+// through the caches). Rows of other alignments take unaligned stores (100000 x 770 bf16: 32 us; element by element
+// 100).
 template <typename T>
 __global__ void __launch_bounds__(256) k_mxfp4_dequantize(int64_t total, int G, int K, int KB,
                                                           const uint8_t* __restrict__ codes,
@@ -127,7 +128,9 @@ __global__ void __launch_bounds__(256) k_mxfp4_dequantize(int64_t total, int G, 
 #pragma unroll
     for (int x = 0; x < 8; ++x) e[x] = from_f32<T>(p[x >> 1][x & 1] * f);
     T* o = out + row[i] * ldo + c[i];
-    if (vec && c[i] + 8 <= K) {
+    if (!vec && c[i] + 8 <= K) {
+      __builtin_memcpy(o, e, sizeof(e));
+    } else if (vec && c[i] + 8 <= K) {
       u32x4 q[sizeof(e) / 16];
       __builtin_memcpy(q, e, sizeof(e));
 #pragma unroll
@@ -339,7 +342,24 @@ __device__ __forceinline__ void tile_of(const MxArgs& a, int v, int64_t& m0, int
   n0 = (int64_t)(cg * a.gn + inc % gn) * MX_T;
 }
 
-// DW: KB is a multiple of 4 and the scales are 4-byte aligned, so a row's scales come by LDS-DMA in words
+// Four scales from p on of a matrix's n at base, at any alignment; in the place of bytes past the end, anything.
+__device__ __forceinline__ uint32_t word_at(const uint8_t* p, const uint8_t* base, int64_t n) {
+  uint32_t w = 0;
+  if (n >= 4) {
+    const uint8_t* last = base + n - 4;
+    const uint8_t* q = p < last ? p : last;
+    __builtin_memcpy(&w, q, 4);
+    return w >> (8 * (int)(p - q));
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (p + i < base + n) w |= (uint32_t)p[i] << (8 * i);
+  return w;
+}
+
+// DW: KB is a multiple of 4 and the scales are 4-byte aligned, so a row's scales come by LDS-DMA in words; without,
+// a thread a row loads them as unaligned words and writes them to LDS (8192 x 8192 x 4064: 260 us, in bytes 485; with
+// aligned rows 8192 x 8192 x 4096 takes 204)
 template <typename T, bool DW>
 __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
   typedef MxMap<T> Map;
@@ -385,15 +405,11 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
           8 * kt, 0, 0);
   };
   uint32_t pend[2] = {0, 0};  // !DW: this thread's row's scales of the stage on its way
-  auto scale_bytes = [&](int kt) {
+  auto scale_words = [&](int kt) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
-      pend[d] = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = 8 * kt + 4 * d + i;
-        pend[d] |= (uint32_t)(srow < rows && at < KB ? sbase[so[0] + at] : 127) << (8 * i);
-      }
+      const int at = 8 * kt + 4 * d;
+      pend[d] = srow < rows && at < KB ? word_at(sbase + so[0] + at, isw ? a.ws : a.as, (isw ? a.N : a.M) * KB) : 0x7F7F7F7Fu;
     }
   };
   // fragment reads: the permutation does not depend on i, and block 4 h + g is slot (g ^ key) ^ 4 h
@@ -406,7 +422,7 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
   aim(m0, n0, true);
 #pragma unroll
   for (int p = 0; p < 10; ++p) piece(0, 0, p);
-  if (!DW) scale_bytes(0);
+  if (!DW) scale_words(0);
   while (true) {
     f32x4 acc[4][4];
 #pragma unroll
@@ -448,7 +464,7 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
         if (nv < tiles) tile_of(a, nv, m1, n1);
         aim(m1, n1, nv < tiles);
       }
-      if (!DW) scale_bytes(next);
+      if (!DW) scale_words(next);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -505,8 +521,9 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
 // U steps of K in flight; the A rows come from the caches. Bound by the read of W for few rows (1 x 1M x 768 88 us,
 // 4.7 TB/s; 1 x 100000 x 4096 41 us, 5.3 TB/s), by the A fragments' way through the caches for many (64 x 1M x 768
 // 231 us, 2.9 TB/s with the result). DW: a row's four scales of
-// a step are one word; the four lanes of a row load the words of four steps and trade them (a byte a lane and
-// step took 66 instead of 41 us at 1 x 100000 x 4096).
+// a step are an aligned word; the four lanes of a row load the words of four steps and trade them (a byte a lane and
+// step took 66 instead of 41 us at 1 x 100000 x 4096). Without, a lane loads its bytes (unaligned words took 100
+// instead of 92 us at 1 x 1M x 736).
 template <typename T, int MT, int NT, bool DW>
 __global__ void __launch_bounds__(256) k_mxfp4_skinny(MxArgs a) {
   constexpr int U = NT == 4 ? (MT == 4 ? 1 : 2) : MT == 4 ? 2 : 4;
@@ -655,12 +672,11 @@ extern "C" int rf_mxfp4_quantize(int dtype, int M, int K, const void* x, int64_t
   RF_REQUIRE((reinterpret_cast<uintptr_t>(x) & (es - 1)) == 0 && aligned16(codes),
              "rf_mxfp4_quantize: misaligned rows or codes");
   const int KB = (K + 31) / 32, sh = lane_shift(K);
-  const bool vec = aligned16(x) && ldx * es % 16 == 0;
   const int64_t blocks = (((int64_t)M << sh) + 255) / 256;
   RF_REQUIRE(blocks * 256 <= 0xFFFFFFFFll, "rf_mxfp4_quantize: %d rows are too many for a launch", M);
   hipStream_t st = as_stream(stream);
 #define MXQ(T)                                                                                                      \
-  k_mxfp4_quantize<T><<<(unsigned)blocks, 256, 0, st>>>(M, K, KB, (const T*)x, ldx, sh, vec, eps, codes, scales, rnorm)
+  k_mxfp4_quantize<T><<<(unsigned)blocks, 256, 0, st>>>(M, K, KB, (const T*)x, ldx, sh, eps, codes, scales, rnorm)
   if (dtype == RF_F32) MXQ(float);
   else if (dtype == RF_BF16) MXQ(bf16);
   else MXQ(f16);

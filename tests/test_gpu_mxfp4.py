@@ -174,6 +174,20 @@ def test_product_of_few_rows_and_many_columns(dev, M, N, K):
     test_product(dev, torch.float32, M, N, K)
 
 
+@pytest.mark.parametrize("M", [3, 100])
+def test_scales_of_any_alignment(dev, M):
+    """Tables of fewer than four scale bytes, and slices of a table, whose scales start anywhere."""
+    for K in (20, 50, 96):
+        test_product(dev, torch.float32, M, 1, K)
+    w = ops.mxfp4_quantize(rows_of(dev, torch.bfloat16, 300, 224, 2))
+    a = ops.mxfp4_quantize(rows_of(dev, torch.bfloat16, M + 5, 224, 3))
+    whole = ops.mxfp4_gemm(a, w)
+    for lo, hi in ((1, 300), (2, 131), (299, 300), (7, 140)):
+        part = ops.Mxfp4(w.codes[lo:hi], w.scales[lo:hi], 224)
+        assert torch.equal(ops.mxfp4_gemm(ops.Mxfp4(a.codes[5:], a.scales[5:], 224), part), whole[5:, lo:hi])
+        assert torch.equal(ops.mxfp4_dequantize(part), ops.mxfp4_dequantize(w)[lo:hi])
+
+
 def test_product_quantises_rows_on_the_way(dev):
     for dt in DTYPES:
         x = rows_of(dev, dt, 70, 200, 5, "offset")
