@@ -33,7 +33,8 @@ template <typename T>
 __device__ __forceinline__ void load8(const T* x, int c, int K, float (&v)[8]) {
   if (c + 8 <= K) {
     T e[8];
-    __builtin_memcpy(e, x + c, sizeof(e));  // 16 bytes at any alignment (element by element 100000 x 770 bf16 took 90 us instead of 39)
+    // 16 bytes at any alignment (element by element 100000 x 770 bf16 took 90 us instead of 39)
+    __builtin_memcpy(e, x + c, sizeof(e));
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
   } else {
@@ -239,7 +240,9 @@ struct MxVec {
         bias[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, col(g, i) * 4, 0, 0));
     }
   }
-  static __device__ __forceinline__ int col(int g, int i) { return (i / (NV / 4)) * 4 * NV + NV * g + 4 * (i % (NV / 4)); }
+  static __device__ __forceinline__ int col(int g, int i) {
+    return (i / (NV / 4)) * 4 * NV + NV * g + 4 * (i % (NV / 4));
+  }
 };
 
 // A wave's 64 x 64 results to rows mw.., columns nw..: acc[i][j] holds columns MxMap::wrow(i, 4 g ..) of row
@@ -307,6 +310,9 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, int64_t mw, int64_t
 // epilogue); two workgroups a CU. W is the matrix instruction's first operand, so that a lane's results are
 // neighbours in a row of C; with 16-bit results the W rows of a pair of instructions are interleaved by fours,
 // so that a lane holds eight neighbours.
+// For short K the stores bound it (4096 x 125000 x 768 fp32: 413 us, 5.0 TB/s of results; 4915 x 50265 x 768 bf16 166 us,
+// where stores alone take 108); for long K the fragments' and the LDS-DMA's way through LDS beside the matrix
+// instructions (8192^3: 376 us, 2.9 PFLOP/s). Loads two steps ahead, with a second barrier a step, took 5% longer.
 // Rows of a stage are 128 bytes; their 16-byte slots are permuted by three bits of the row, so that eight
 // neighbouring lanes of a fragment read cover all banks.
 constexpr int MX_T = 128;
@@ -409,7 +415,8 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
       const int at = 8 * kt + 4 * d;
-      pend[d] = srow < rows && at < KB ? word_at(sbase + so[0] + at, isw ? a.ws : a.as, (isw ? a.N : a.M) * KB) : 0x7F7F7F7Fu;
+      pend[d] = 0x7F7F7F7Fu;
+      if (srow < rows && at < KB) pend[d] = word_at(sbase + so[0] + at, isw ? a.ws : a.as, (isw ? a.N : a.M) * KB);
     }
   };
   // fragment reads: the permutation does not depend on i, and block 4 h + g is slot (g ^ key) ^ 4 h
