@@ -279,7 +279,6 @@ __device__ __attribute__((noinline)) int collect_exact(const Src src, int k, int
 // Where more than CAP entries pass (many equal values, or the best all in few threads) the exact search follows.
 template <int TPB, typename Src>
 __device__ __forceinline__ int collect(const Src& src, bool nan, int k, int64_t n, SelectLds<TPB>& s) {
-  const int t = threadIdx.x;
   auto take = [&](uint64_t e) {
     const int at = atomicAdd(&s.count, 1);
     if (at < SelectLds<TPB>::CAP) s.cand[at] = e;
@@ -664,9 +663,10 @@ struct LpBwdArgs {
 
 // One slice of a row: read, e^t / s, write. The listed entries are then written again by one thread each
 // (after a barrier; the first of equal ids adds all their weights in list order), so nothing is added
-// atomically. HBM bound: 4915 x 50265 bf16 175 us (5.6 TB/s), 128 x 1M fp32 211 (4.9 TB/s); LB_R chunks a thread
+// atomically. HBM bound: 4915 x 50265 bf16 168 us (5.9 TB/s), 128 x 1M fp32 207 (4.9 TB/s); LB_R chunks a thread
 // keep enough loads in flight beside the stores.
-template <typename T, int TPB, bool ENT>
+// PAST: the gradient is written past the caches.
+template <typename T, int TPB, bool ENT, bool PAST>
 __global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __restrict__ logits,
                                                          T* __restrict__ dlogits) {
   constexpr int V = Row<T>::V;
@@ -740,7 +740,8 @@ __global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __re
       if (c0 >= 0 && c0 + V <= a.N) {
         u32x4 w;
         __builtin_memcpy(&w, o, 16);
-        *reinterpret_cast<u32x4*>(dx + c0) = w;
+        if (PAST) __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(dx + c0));
+        else *reinterpret_cast<u32x4*>(dx + c0) = w;
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -873,12 +874,18 @@ static int lp_backward(const char* name, int dtype, const LpBwdArgs& in, const v
   RF_REQUIRE((int64_t)a.M * a.S * tpb <= 0xFFFFFFFFll, "%s: %d rows of %d slices are too many for a launch", name,
              a.M, a.S);
   const unsigned grid = (unsigned)((int64_t)a.M * a.S);
-#define LB_K(T, TPB, ENT) k_logprobs_bwd<T, TPB, ENT><<<grid, TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits)
-#define LB_T(T)                                 \
-  if (tpb == 64 && a.g_ent) LB_K(T, 64, true);  \
-  else if (tpb == 64) LB_K(T, 64, false);       \
-  else if (a.g_ent) LB_K(T, 256, true);         \
-  else LB_K(T, 256, false)
+  // A gradient that the products behind it find in the caches (256 MB) is kept there, a larger one only pushes the
+  // next logits out: distillation of 4915 x 50265 bf16 forward and backward 287 us, 302 through the caches, with both
+  // products behind it 824 and 838, 2457 rows (247 MB) 643 and 646; but 1200 rows (121 MB) 465 and 420.
+  const bool past = (int64_t)a.M * a.N * es > (int64_t)192 << 20;
+#define LB_K(T, TPB, ENT)                                                                                              \
+  if (past) k_logprobs_bwd<T, TPB, ENT, true><<<grid, TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits);                \
+  else k_logprobs_bwd<T, TPB, ENT, false><<<grid, TPB, 0, st>>>(a, (const T*)logits, (T*)dlogits)
+#define LB_T(T)                                    \
+  if (tpb == 64 && a.g_ent) { LB_K(T, 64, true); } \
+  else if (tpb == 64) { LB_K(T, 64, false); }      \
+  else if (a.g_ent) { LB_K(T, 256, true); }        \
+  else { LB_K(T, 256, false); }
   if (dtype == RF_F32) { LB_T(float); }
   else if (dtype == RF_BF16) { LB_T(bf16); }
   else { LB_T(f16); }

@@ -533,3 +533,19 @@ def test_history_ids_outside_the_catalog_leave_out_nothing(dev):
     with pytest.raises(ValueError):
         m.distill_loss(torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.long),
                        candidates=torch.zeros(2, 3, dtype=torch.long))
+
+
+@pytest.mark.parametrize("M,N", [(2100, 50265), (110000, 1000)])
+def test_large_gradients_are_those_of_their_parts(dev, M, N):
+    """A gradient larger than the caches hold is written another way: bit by bit that of a few of its rows."""
+    x = logits_of(dev, torch.bfloat16, M, N, 7)
+    tok = torch.randint(0, N, (M, 2), device=dev)
+    g, gh = torch.randn(M, 2, device=dev), torch.randn(M, device=dev)
+    r = ops.token_logprobs(x, tok, want_entropy=True, want_stats=True)
+    d = ops.token_logprobs_bwd(x, r.stats, tok, g, r.entropy, gh)
+    for lo in (0, M - 40):
+        p = slice(lo, lo + 40)
+        part = ops.token_logprobs_bwd(x[p], r.stats[p], tok[p], g[p], r.entropy[p], gh[p])
+        assert torch.equal(d[p], part)
+        want, size = ref_grad(x[p], 1.0, tok[p], g[p], gh[p])
+        close_grad(part, want, size)
