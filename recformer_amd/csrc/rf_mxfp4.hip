@@ -285,7 +285,10 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, int64_t mw, int64_t
         even_row[x] = odd ? n1 : w[0][x];
         odd_row[x] = odd ? w[1][x] : n0;
       }
-      if (!EDGE) {  // non-temporal: read by nobody soon, and the tables stay in L2
+      // non-temporal: the tables stay in L2 (512 x 100000 x 768 fp32: 48 us, 83 without; what a reader that finds the
+      // result in no cache loses is less or about as much: with the top 10 of each row behind it 129 and 122, 4096 x
+      // 125000 905 and 1032)
+      if (!EDGE) {
         __builtin_amdgcn_raw_buffer_store_b128(even_row, rc, at + q * 64, 0, 2);
         __builtin_amdgcn_raw_buffer_store_b128(odd_row, rc, at + row + q * 64, 0, 2);
       } else {
