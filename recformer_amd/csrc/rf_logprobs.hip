@@ -272,7 +272,6 @@ __device__ __attribute__((noinline)) int collect_exact(const Src src, int k, int
   return min(s.count, SelectLds<TPB>::CAP);
 }
 
-
 // Collects into s.cand what passes s.tau, at least min(k, n) entries and among them the k best, and returns how
 // many. src.each(tau, f) calls f(entry) for every entry of the calling thread whose key is >= tau,
 // src.again().all(f) for all its entries; nan: some value is NaN (the float compares of src.each would miss it).
