@@ -991,7 +991,7 @@ class TokenLogprobs(NamedTuple):
 def _run(fn, what: str, ref: torch.Tensor, *args) -> None:
     """fn(*args, stream) on ref's device (made current for the call where it is not) and its current stream."""
     dev = ref.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
@@ -1030,14 +1030,15 @@ def _row_list(what: str, t: torch.Tensor, logits: torch.Tensor, dtype: torch.dty
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _like_rows(logits: torch.Tensor, ld: int) -> Tuple[torch.Tensor, int]:
-    """An empty (M, N) tensor whose rows are aligned as the logits' rows are (contiguous where theirs allow it)."""
-    M, N = logits.shape
-    es = logits.element_size()
+def _like_rows(rows, logits: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """An empty (M, N) tensor whose rows are aligned as the logits' rows are (contiguous where theirs allow it), and
+    its row stride; rows: _logit_rows of these logits."""
+    code, M, N, at, ld, _ = rows
+    es = 4 if code == RF_F32 else 2
     ldd = N + (ld - N) % (16 // es)
-    off = logits.data_ptr() % 16 // es
+    off = at % 16 // es
     if off == 0 and ldd == N:
-        return torch.empty(M, N, dtype=logits.dtype, device=logits.device), ldd
+        return torch.empty((M, N), dtype=logits.dtype, device=logits.device), ldd
     buf = torch.empty(off + M * ldd, dtype=logits.dtype, device=logits.device)
     return buf.as_strided((M, N), (ldd, 1), off), ldd
 
@@ -1057,27 +1058,31 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     (rf_token_logprobs_fwd): of the given tokens ((M,) or (M, C) ids, C <= 1024; ignore_index gives 0, any
     other id outside [0, N) NaN), the entropy, and the k <= 256 best alternatives (largest logit first, the
     lower id first among equals). Masked columns are -inf; a row of nothing else gives -inf, entropy 0."""
-    lib = _lib.load()
     rows = _logit_rows("token_logprobs", logits, inv_temp)
-    code, M, N = rows[:3]
+    M, N = rows[1:3]
     if not 0 <= k <= min(N, 256):
         raise ValueError(f"token_logprobs: k={k} must be in [0, min(N, 256)]")
-    dev, f32 = logits.device, torch.float32
-    ids = logp = None
-    C = 0
+    ids = shape = None
     if tokens is not None:
-        ids = _token_ids("token_logprobs: tokens", tokens, logits)
-        C = ids.shape[1]
-        logp = torch.empty(tokens.shape, dtype=f32, device=dev)
+        ids, shape = _token_ids("token_logprobs: tokens", tokens, logits), tokens.shape
     elif not (k or want_entropy or want_stats):
         raise ValueError("token_logprobs: no output requested")
+    return _logprobs(rows, logits, ids, shape, k, int(ignore_index), want_entropy, want_stats)
+
+
+def _logprobs(rows, logits, ids, shape, k: int, ignore: int, want_entropy: bool, want_stats: bool) -> TokenLogprobs:
+    """The checked call; rows: _logit_rows of these logits, ids: _token_ids of tokens of the given shape, or None."""
+    lib = _lib.load()
+    code, M, N = rows[:3]
+    dev, f32 = logits.device, torch.float32
+    logp = torch.empty(shape, dtype=f32, device=dev) if ids is not None else None
     ent = torch.empty(M, dtype=f32, device=dev) if want_entropy else None
     tv = torch.empty(M, k, dtype=f32, device=dev) if k else None
     ti = torch.empty(M, k, dtype=torch.int64, device=dev) if k else None
     stats = torch.empty(M, 4, dtype=f32, device=dev) if want_stats else None
     ws = _logprobs_ws(lib, code, M, N, k, dev)
-    _run(lib.rf_token_logprobs_fwd, "rf_token_logprobs_fwd", logits, *rows, _p(ids), C, int(ignore_index), k, _p(logp),
-         _p(ent), _p(tv), _p(ti), _p(stats), _p(ws))
+    _run(lib.rf_token_logprobs_fwd, "rf_token_logprobs_fwd", logits, *rows, _p(ids), 0 if ids is None else ids.shape[1],
+         ignore, k, _p(logp), _p(ent), _p(tv), _p(ti), _p(stats), _p(ws))
     return TokenLogprobs(logp, ent, tv, ti, stats)
 
 
@@ -1109,7 +1114,7 @@ def token_logprobs_bwd(logits: torch.Tensor, stats: torch.Tensor, tokens: Option
 
 def _logprobs_grad(rows, logits, stats, ids, C: int, ignore: int, g_logp, entropy, g_entropy) -> torch.Tensor:
     """The checked call; rows: _logit_rows of these logits."""
-    out, ldd = _like_rows(logits, rows[4])
+    out, ldd = _like_rows(rows, logits)
     _run(_lib.load().rf_token_logprobs_bwd, "rf_token_logprobs_bwd", logits, *rows, _p(stats), _p(ids), C, ignore,
          _p(g_logp), _p(entropy), _p(g_entropy), _p(out), ldd)
     return out
@@ -1137,22 +1142,24 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids
     one-element device tensors, with n the rows that use a slot (nan if none does). teacher_logits may be
     log probabilities."""
     rows = _logit_rows("topk_distill", logits, inv_temp)
-    return _distill(rows, logits, *_teacher("topk_distill", logits, teacher_logits, teacher_ids), scale)
+    loss, buf = _distill(rows, logits, *_teacher("topk_distill", logits, teacher_logits, teacher_ids), scale)
+    M = rows[1]
+    return buf[4 * M:5 * M], buf[:4 * M].view(M, 4), loss, buf[5 * M]
 
 
 def _distill(rows, logits, val, ids, scale: float):
-    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them."""
+    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them. (loss, fp32 buffer of
+    the stats (M, 4), the rows' losses (M,) and coef)."""
     lib = _lib.load()
     code, M, N = rows[:3]
     dev, f32 = logits.device, torch.float32
-    per_row = torch.empty(M, dtype=f32, device=dev)
-    stats = torch.empty(M, 4, dtype=f32, device=dev)
+    buf = torch.empty(5 * M + 1, dtype=f32, device=dev)
     loss = torch.empty((), dtype=f32, device=dev)
-    coef = torch.empty((), dtype=f32, device=dev)
     ws = _logprobs_ws(lib, code, M, N, 0, dev)
-    _run(lib.rf_topk_distill_fwd, "rf_topk_distill_fwd", logits, *rows, _p(val), _p(ids), ids.shape[1], float(scale),
-         _p(per_row), _p(stats), _p(loss), _p(coef), _p(ws))
-    return per_row, stats, loss, coef
+    at = buf.data_ptr()
+    _run(lib.rf_topk_distill_fwd, "rf_topk_distill_fwd", logits, *rows, val.data_ptr(), ids.data_ptr(), ids.shape[1],
+         float(scale), at + 16 * M, at, loss.data_ptr(), at + 20 * M, _p(ws))
+    return loss, buf
 
 
 def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: torch.Tensor,
@@ -1166,14 +1173,15 @@ def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: 
     for t in (g, coef):
         if t.numel() != 1 or t.dtype != torch.float32 or t.get_device() != logits.get_device():
             raise ValueError("topk_distill_bwd: g and coef are one-element fp32 tensors beside the logits")
-    return _distill_grad(rows, logits, stats, val, ids, g, coef)
+    return _distill_grad(rows, logits, stats.data_ptr(), val, ids, g, coef.data_ptr())
 
 
-def _distill_grad(rows, logits, stats, val, ids, g, coef) -> torch.Tensor:
-    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them."""
-    out, ldd = _like_rows(logits, rows[4])
-    _run(_lib.load().rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, *rows, stats.data_ptr(), val.data_ptr(),
-         ids.data_ptr(), ids.shape[1], g.data_ptr(), coef.data_ptr(), out.data_ptr(), ldd)
+def _distill_grad(rows, logits, stats: int, val, ids, g, coef: int) -> torch.Tensor:
+    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them, stats and coef
+    addresses."""
+    out, ldd = _like_rows(rows, logits)
+    _run(_lib.load().rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, *rows, stats, val.data_ptr(), ids.data_ptr(),
+         ids.shape[1], g.data_ptr(), coef, out.data_ptr(), ldd)
     return out
 
 

@@ -521,6 +521,15 @@ def _differentiable_once(backward):
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
+def _rows_again(ctx, logits):
+    """The forward's ops._logit_rows of saved logits; hooks on saved tensors may have moved them, or changed their
+    rows' stride."""
+    rows = ctx.rows
+    if logits.data_ptr() != rows[3] or logits.stride(0) != ctx.ld:
+        rows = ops._logit_rows("saved logits", logits, rows[-1])
+    return rows
+
+
 class _TokenLogprobs(torch.autograd.Function):
     """Log probabilities of given entries and the entropy of softmax(logits * inv_temp), one pass over the
     logits forward (rf_token_logprobs_fwd) and one backward (rf_token_logprobs_bwd, which recomputes the
@@ -528,10 +537,11 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, inv_temp: float, ignore_index: int):
-        r = ops.token_logprobs(logits, tokens, inv_temp=inv_temp, ignore_index=ignore_index, want_entropy=True,
-                               want_stats=True)
-        ctx.save_for_backward(logits, tokens, r.stats, r.entropy)
-        ctx.args = (inv_temp, ignore_index)
+        rows = ops._logit_rows("token_logprobs_train", logits, inv_temp)
+        ids = ops._token_ids("token_logprobs_train: tokens", tokens, logits)
+        r = ops._logprobs(rows, logits, ids, tokens.shape, 0, ignore_index, True, True)
+        ctx.save_for_backward(logits, ids, r.stats, r.entropy)
+        ctx.rows, ctx.ld, ctx.ignore = rows, logits.stride(0), ignore_index
         ctx.set_materialize_grads(False)
         return r.logp, r.entropy
 
@@ -540,9 +550,14 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy):
         if not ctx.needs_input_grad[0] or (g_logp is None and g_entropy is None):
             return None, None, None, None
-        logits, tokens, stats, entropy = ctx.saved_tensors
-        inv_temp, ign = ctx.args
-        return ops.token_logprobs_bwd(logits, stats, tokens, g_logp, entropy, g_entropy, inv_temp, ign), None, None, None
+        logits, ids, stats, entropy = ctx.saved_tensors
+        rows = _rows_again(ctx, logits)
+        if g_logp is not None and not g_logp.is_contiguous():
+            g_logp = g_logp.contiguous()
+        if g_entropy is not None and not g_entropy.is_contiguous():
+            g_entropy = g_entropy.contiguous()
+        C = 0 if g_logp is None else ids.shape[1]
+        return ops._logprobs_grad(rows, logits, stats, ids, C, ctx.ignore, g_logp, entropy, g_entropy), None, None, None
 
 
 class _TopkDistill(torch.autograd.Function):
@@ -553,9 +568,9 @@ class _TopkDistill(torch.autograd.Function):
     def forward(ctx, logits, teacher_logits, teacher_ids, temp: float):
         rows = ops._logit_rows("topk_distill_train", logits, 1.0 / temp)
         val, ids = ops._teacher("topk_distill_train", logits, teacher_logits, teacher_ids)
-        _, stats, loss, coef = ops._distill(rows, logits, val, ids, temp * temp)
-        ctx.save_for_backward(logits, val, ids, stats, coef)
-        ctx.inv_temp = rows[-1]
+        loss, buf = ops._distill(rows, logits, val, ids, temp * temp)
+        ctx.save_for_backward(logits, val, ids, buf)
+        ctx.rows, ctx.ld = rows, logits.stride(0)
         return loss
 
     @staticmethod
@@ -563,10 +578,10 @@ class _TopkDistill(torch.autograd.Function):
     def backward(ctx, g):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
-        logits, val, ids, stats, coef = ctx.saved_tensors
-        # checked again: hooks on saved tensors may give back rows of another stride
-        rows = ops._logit_rows("topk_distill_train", logits, ctx.inv_temp)
-        return ops._distill_grad(rows, logits, stats, val, ids, g, coef), None, None, None
+        logits, val, ids, buf = ctx.saved_tensors
+        rows = _rows_again(ctx, logits)
+        at = buf.data_ptr()
+        return ops._distill_grad(rows, logits, at, val, ids, g, at + 20 * rows[1]), None, None, None
 
 
 def token_logprobs_train(logits: torch.Tensor, tokens: torch.Tensor, inv_temp: float = 1.0, ignore_index: int = -100):
