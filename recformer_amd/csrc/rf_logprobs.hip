@@ -773,8 +773,8 @@ static int lp_vec(int dtype) { return dtype == RF_F32 ? 4 : 8; }
 // against 8 KB slices: 64 x 10000 fp32 top 50 8.7 and 13.6 us, 300 x 50265 top 20 15.0 and 21.7; the other way
 // only for a row or two without alternatives, 1 x 50265 7.5 and 6.5). Rows that are joined anyway, and fewer than
 // two workgroups a CU, are cut further, down to LP_MIN_CHUNKS chunks (1 x 70000: 6.4 us, 9.1 uncut, 4 x 1M bf16
-// 7.3 and 11.0), as long as the join reads at most LP_JOIN entries a row (1 x 1M top 256 in 64 slices instead of
-// 31: 76 and 62 us, 4 x 1M top 50 in 128 instead of 31: 20.0 and 18.5).
+// 7.3 and 11.0), as long as the join reads at most LP_JOIN entries a row (1 x 1M fp32 top 50 17.6 us, 27.9 with
+// 16384; top 256 34.1 and 38.8).
 constexpr int LP_CUS = 256, LP_MIN_CHUNKS = 512, LP_JOIN = 4096;
 static void lp_plan(int dtype, int M, int N, int k, int* S, int* cps) {
   const int V = lp_vec(dtype);
@@ -808,8 +808,8 @@ static void lp_launch(const LpArgs& a, const void* x, hipStream_t st) {
   else if (tpb == 256) k_logprobs<T, 256, ENT, TOP, TEACH><<<grid, 256, 0, st>>>(a, p);
   else k_logprobs<T, 1024, ENT, TOP, TEACH><<<grid, 1024, 0, st>>>(a, p);
   if (a.S > 1) {
-    // 256 threads for short lists (1 x 50265 in 12 slices, top 5: 10.2 and 11.0 us), 1024 for long ones (4 x 1M, 128
-    // lists of 50: 26.7 and 19.9)
+    // 256 threads for short lists (1 x 100000 bf16 top 5: 10.0 us, 10.7 with 1024), 1024 for long ones (1 x 1M fp32 top
+    // 50: 17.5 us, 21.6 with 256)
     if (!TOP || (a.S * a.k <= 2048 && a.k <= 64)) k_logprobs_join<T, 256, TOP, TEACH><<<a.M, 256, 0, st>>>(a, p);
     else k_logprobs_join<T, 1024, TOP, TEACH><<<a.M, 1024, 0, st>>>(a, p);
   }
