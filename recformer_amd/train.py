@@ -521,13 +521,27 @@ def _differentiable_once(backward):
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
-def _rows_again(ctx, logits):
-    """The forward's ops._logit_rows of saved logits; hooks on saved tensors may have moved them, or changed their
-    rows' stride."""
-    rows = ctx.rows
-    if logits.data_ptr() != rows[3] or logits.stride(0) != ctx.ld:
+def _saved_again(ctx, logits, *lists):
+    """(the forward's ops._logit_rows, logits, lists) of the saved logits and of the lists and buffers beside them,
+    contiguous in the forward. Hooks on saved tensors may have moved them or changed their strides; what they left on
+    another device, or gave another type or shape, is refused before it reaches a kernel by its address."""
+    dev, layout, rows = ctx.layout[0], ctx.layout[1:], ctx.rows
+    for t, (dtype, shape) in zip((logits, *lists), layout):
+        if t.get_device() != dev or t.dtype != dtype or t.shape != shape:
+            raise ValueError(f"saved tensors: {tuple(t.shape)} {t.dtype} on {t.device} in the place of "
+                             f"{tuple(shape)} {dtype} of the forward's device")
+    if logits.data_ptr() != rows[3] or logits.stride() != ctx.strides:
+        if logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]:
+            logits = logits.contiguous()
         rows = ops._logit_rows("saved logits", logits, rows[-1])
-    return rows
+    return rows, logits, [t if t.is_contiguous() else t.contiguous() for t in lists]
+
+
+def _save_rows(ctx, rows, logits, *lists):
+    """Saves the logits and the lists and buffers beside them for _saved_again; rows: ops._logit_rows of the logits."""
+    ctx.save_for_backward(logits, *lists)
+    ctx.rows, ctx.strides = rows, logits.stride()
+    ctx.layout = (logits.get_device(), *((t.dtype, t.shape) for t in (logits, *lists)))
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -540,8 +554,8 @@ class _TokenLogprobs(torch.autograd.Function):
         rows = ops._logit_rows("token_logprobs_train", logits, inv_temp)
         ids = ops._token_ids("token_logprobs_train: tokens", tokens, logits)
         r = ops._logprobs(rows, logits, ids, tokens.shape, 0, ignore_index, True, True)
-        ctx.save_for_backward(logits, ids, r.stats, r.entropy)
-        ctx.rows, ctx.ld, ctx.ignore = rows, logits.stride(0), ignore_index
+        _save_rows(ctx, rows, logits, ids, r.stats, r.entropy)
+        ctx.ignore = ignore_index
         ctx.set_materialize_grads(False)
         return r.logp, r.entropy
 
@@ -550,8 +564,7 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy):
         if not ctx.needs_input_grad[0] or (g_logp is None and g_entropy is None):
             return None, None, None, None
-        logits, ids, stats, entropy = ctx.saved_tensors
-        rows = _rows_again(ctx, logits)
+        rows, logits, (ids, stats, entropy) = _saved_again(ctx, *ctx.saved_tensors)
         if g_logp is not None and not g_logp.is_contiguous():
             g_logp = g_logp.contiguous()
         if g_entropy is not None and not g_entropy.is_contiguous():
@@ -569,8 +582,7 @@ class _TopkDistill(torch.autograd.Function):
         rows = ops._logit_rows("topk_distill_train", logits, 1.0 / temp)
         val, ids = ops._teacher("topk_distill_train", logits, teacher_logits, teacher_ids)
         loss, buf = ops._distill(rows, logits, val, ids, temp * temp)
-        ctx.save_for_backward(logits, val, ids, buf)
-        ctx.rows, ctx.ld = rows, logits.stride(0)
+        _save_rows(ctx, rows, logits, val, ids, buf)
         return loss
 
     @staticmethod
@@ -578,8 +590,7 @@ class _TopkDistill(torch.autograd.Function):
     def backward(ctx, g):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
-        logits, val, ids, buf = ctx.saved_tensors
-        rows = _rows_again(ctx, logits)
+        rows, logits, (val, ids, buf) = _saved_again(ctx, *ctx.saved_tensors)
         at = buf.data_ptr()
         return ops._distill_grad(rows, logits, at, val, ids, g, at + 20 * rows[1]), None, None, None
 

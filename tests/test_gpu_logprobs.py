@@ -549,3 +549,36 @@ def test_large_gradients_are_those_of_their_parts(dev, M, N):
         assert torch.equal(d[p], part)
         want, size = ref_grad(x[p], 1.0, tok[p], g[p], gh[p])
         close_grad(part, want, size)
+
+
+def _every_other(t):
+    """t's numbers in every other element of a larger buffer."""
+    buf = torch.zeros(*t.shape[:-1], 2 * t.shape[-1], dtype=t.dtype, device=t.device)
+    buf[..., ::2] = t
+    return buf[..., ::2]
+
+
+@pytest.mark.parametrize("N", [50, 4100])
+def test_saved_tensor_hooks_that_move_the_lists(dev, N):
+    """Hooks that hand every saved tensor back with gaps between its elements: the same gradient; hooks that leave them
+    on the host: an error."""
+    x = logits_of(dev, torch.float32, 5, N, 3)
+    ids = torch.randint(0, N, (5, 4), device=dev)
+    tl = torch.randn(5, 4, device=dev)
+    lists = [lambda y: sum(t.sum() for t in train.token_logprobs_train(y, ids, 1.3)),
+             lambda y: train.topk_distill_train(y, tl, ids, 2.0)]
+    for fn in lists:
+        leaf = x.clone().requires_grad_()
+        want, = torch.autograd.grad(fn(leaf), leaf)
+        with torch.autograd.graph.saved_tensors_hooks(_every_other, lambda t: t):
+            out = fn(leaf)
+        got, = torch.autograd.grad(out, leaf)
+        assert torch.equal(got, want)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
+            out = fn(leaf)
+        with pytest.raises(ValueError):
+            torch.autograd.grad(out, leaf)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
+            out = fn(leaf)
+        got, = torch.autograd.grad(out, leaf)
+        assert torch.equal(got, want)

@@ -142,3 +142,86 @@ def test_signatures_take_what_the_header_declares():
             want = (ctypes.c_void_p if ptr else ctypes.c_float if "float" in a else
                     ctypes.c_int64 if "int64_t" in a else ctypes.c_int)
             assert t is want, (name, a)
+
+
+class Ctx:
+    """An autograd context whose saved tensors may be put in other places, as hooks on saved tensors do."""
+
+    needs_input_grad = (True, False, False, False)
+
+    def save_for_backward(self, *t):
+        self.saved_tensors = t
+
+    def set_materialize_grads(self, on):
+        pass
+
+
+class OnDevice(torch.Tensor):
+    """A host tensor that says it is on device 0."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return t.as_subclass(cls)
+
+    def get_device(self):
+        return 0
+
+
+def _saved_by_forward(monkeypatch, kind, put=lambda t: t):
+    """The context that a forward on 3 rows of 40 leaves, and the calls that its backward makes; no kernel runs."""
+    calls = []
+    x = put(torch.randn(3, 40))
+    ids = put(torch.arange(12).view(3, 4))
+    monkeypatch.setattr(ops, "_dev", lambda *ts: None)
+    monkeypatch.setattr(ops, "_logprobs", lambda *a: ops.TokenLogprobs(put(torch.zeros(3, 4)), put(torch.zeros(3)), None,
+                                                                       None, put(torch.arange(12.0).view(3, 4))))
+    monkeypatch.setattr(ops, "_distill", lambda *a: (put(torch.zeros(())), put(torch.arange(16.0))))
+    monkeypatch.setattr(ops, "_logprobs_grad", lambda rows, *a: calls.append((rows, *a)))
+    monkeypatch.setattr(ops, "_distill_grad", lambda rows, *a: calls.append((rows, *a)))
+    ctx = Ctx()
+    if kind == "logprobs":
+        train._TokenLogprobs.forward(ctx, x, ids, 1.0, -100)
+        back = lambda: train._TokenLogprobs.backward(ctx, torch.ones(3, 4), torch.ones(3))
+    else:
+        train._TopkDistill.forward(ctx, x, put(torch.randn(3, 4)), ids, 2.0)
+        back = lambda: train._TopkDistill.backward(ctx, torch.ones(()))
+    return ctx, calls, back
+
+
+def _strided(t):
+    """The same numbers, every other element of a larger buffer."""
+    buf = torch.full((*t.shape[:-1], 2 * t.shape[-1]), -1, dtype=t.dtype)
+    buf[..., ::2] = t
+    return buf[..., ::2]
+
+
+@pytest.mark.parametrize("kind", ["logprobs", "distill"])
+def test_saved_lists_with_other_strides_reach_the_gradient_in_order(monkeypatch, kind):
+    ctx, calls, back = _saved_by_forward(monkeypatch, kind)
+    with torch.no_grad():
+        back()
+        saved = ctx.saved_tensors
+        ctx.saved_tensors = tuple(_strided(t) for t in saved)  # the logits are no row-major view either
+        back()
+    (_, *want), (rows, *got) = calls
+    assert rows[:3] == (0, 3, 40) and rows[3] == got[0].data_ptr() and rows[4] == 40
+    for a, b in zip(want, got):
+        if isinstance(a, torch.Tensor):
+            assert torch.equal(a, b) and b.is_contiguous()
+    assert all(not t.is_contiguous() for t in ctx.saved_tensors)
+
+
+@pytest.mark.parametrize("kind", ["logprobs", "distill"])
+def test_saved_tensors_left_elsewhere_are_refused(monkeypatch, kind):
+    """On another device, or of another type or shape: an error, before anything is launched by their address."""
+    ctx, calls, back = _saved_by_forward(monkeypatch, kind, OnDevice)
+    saved = ctx.saved_tensors
+    with torch.no_grad():
+        back()
+        assert len(calls) == 1
+        for i, t in enumerate(saved):
+            for bad in (t.as_subclass(torch.Tensor), t.to(torch.float64), t[:-1], t.reshape(-1, 1, 1)):
+                ctx.saved_tensors = saved[:i] + (bad,) + saved[i + 1:]
+                with pytest.raises(ValueError):
+                    back()
+    assert len(calls) == 1
