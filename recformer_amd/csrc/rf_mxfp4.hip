@@ -738,8 +738,8 @@ extern "C" int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* 
   a.ac = a_codes; a.as = a_scales; a.wc = w_codes; a.ws = w_scales;
   a.bias = bias; a.ra = ra; a.rw = rw; a.col_scale = col_scale; a.c = C; a.ldc = ldc;
   a.vec = aligned16(C) && ldc * es % 16 == 0;
-  a.nTm = (M + MX_T - 1) / MX_T;
-  a.nTn = (N + MX_T - 1) / MX_T;
+  a.nTm = (int)((a.M + MX_T - 1) / MX_T);
+  a.nTn = (int)((a.N + MX_T - 1) / MX_T);
   // row tiles whose codes fill half of an XCD's 4 MB of L2
   a.gm = (int)std::max<int64_t>(1, std::min<int64_t>(a.nTm, (2 << 20) / ((int64_t)MX_T * a.KB * 16)));
   // column tiles side by side (1, 4, 8: 428, 413, 416 us at 4096 x 125000 x 768 fp32; 8192^3 373, 379, 384)

@@ -1200,23 +1200,32 @@ class Mxfp4(NamedTuple):
         return self.codes.shape[0]
 
 
+def _mxfp4_size(what: str, rows: int, k: int) -> None:
+    """What the entry points take in their C ints."""
+    if rows >= 2 ** 31 or not 1 <= k <= 2 ** 24:
+        raise ValueError(f"{what}: {rows} rows of {k} values (fewer than 2^31 rows, 1 to 2^24 values)")
+
+
 def _mxfp4_check(what: str, q: Mxfp4) -> None:
+    _mxfp4_size(what, q.codes.shape[0], q.k)
     _dev(q.codes, q.scales)
     kb = (q.k + 31) // 32
     for t, name, w in ((q.codes, "codes", kb * 16), (q.scales, "scales", kb)):
         if t.dtype != torch.uint8 or t.dim() != 2 or tuple(t.shape) != (q.codes.shape[0], w) or not t.is_contiguous():
             raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} for k={q.k}: contiguous uint8 (rows, {w})")
-    if q.k < 1 or q.codes.data_ptr() % 16 or q.scales.device != q.codes.device:
-        raise ValueError(f"{what}: k must be positive, codes 16-byte aligned, scales beside them")
+    if q.codes.data_ptr() % 16 or q.scales.device != q.codes.device:
+        raise ValueError(f"{what}: codes must be 16-byte aligned, scales beside them")
 
 
 def _mxfp4_rows(x: torch.Tensor, want_rnorm: bool, eps: float):
     lib = _lib.load()
+    if x.dim() == 2:
+        _mxfp4_size("mxfp4_quantize", *x.shape)
     _dev(x)
     code = dtype_code(x.dtype)
     ld = _rowmajor(x, "x")
     M, K = x.shape
-    if K < 1 or (M > 1 and ld < K):
+    if M > 1 and ld < K:
         raise ValueError(f"mxfp4_quantize: rows of shape {tuple(x.shape)}, strides {x.stride()}")
     kb = (K + 31) // 32
     codes = torch.empty(M, kb * 16, dtype=torch.uint8, device=x.device)

@@ -225,3 +225,26 @@ def test_saved_tensors_left_elsewhere_are_refused(monkeypatch, kind):
                 with pytest.raises(ValueError):
                     back()
     assert len(calls) == 1
+
+
+def test_mxfp4_sizes_past_the_c_ints_are_refused():
+    """2^32 rows would be 0 rows there, 2^32 + 32 columns a row of 32: refused before anything is allocated."""
+    for rows, k in ((2 ** 31, 32), (2 ** 32, 32), (2 ** 32 + 3, 1), (1, 2 ** 24 + 1), (2, 2 ** 32 + 32)):
+        x = torch.empty(rows, k, dtype=torch.bfloat16, device="meta")
+        kb = -(-k // 32)
+        q = ops.Mxfp4(torch.empty(rows, kb * 16, dtype=torch.uint8, device="meta"),
+                      torch.empty(rows, kb, dtype=torch.uint8, device="meta"), k)
+        one = ops.Mxfp4(torch.empty(1, kb * 16, dtype=torch.uint8), torch.empty(1, kb, dtype=torch.uint8), k)
+        for call in (lambda: ops.mxfp4_quantize(x), lambda: ops.mxfp4_quantize(x, want_rnorm=True),
+                     lambda: ops.mxfp4_dequantize(q), lambda: ops.mxfp4_gemm(x, one), lambda: ops.mxfp4_gemm(q, one),
+                     lambda: Mxfp4Catalog.from_items(x)):
+            with pytest.raises(ValueError, match="2\\^31 rows"):
+                call()
+
+
+def test_product_tiles_are_counted_in_64_bits():
+    """Rows next to 2^31: the count of row tiles stays positive, so that too many tiles are seen as such."""
+    lib = _lib.load()
+    for M in (2 ** 31 - 127, 2 ** 31 - 1):
+        assert "too many tiles" in err(lib.rf_mxfp4_gemm(0, M, 1 << 24, 32, A, A, A, A, None, None, None, 1.0, A, 1 << 24,
+                                                         None))
