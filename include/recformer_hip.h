@@ -586,8 +586,8 @@ int rf_mxfp4_quantize(int dtype, int M, int K, const void* x, int64_t ldx, float
 int rf_mxfp4_dequantize(int dtype, int M, int K, const uint8_t* codes, const uint8_t* scales, void* out, int64_t ldo,
                         rf_stream_t stream);
 /* C = A . W^T of two such matrices (M rows and N rows of K), fp32 accumulation, then * ra[m] * col_scale * rw[n]
- * (ra (M) and rw (N) fp32, both or neither: cosine scores) and + bias[n] (fp32 or NULL), rounded once to
- * out_dtype. C: (M, N), row stride ldc, both it and C's address multiples of four elements; rw and bias 16-byte
+ * (ra (M) and rw (N) fp32, both, for cosine scores, or neither: then only * col_scale) and + bias[n] (fp32 or NULL),
+ * rounded once to out_dtype. C: (M, N), row stride ldc, both it and C's address multiples of four elements; rw and bias 16-byte
  * aligned. */
 int rf_mxfp4_gemm(int out_dtype, int M, int N, int K, const uint8_t* a_codes, const uint8_t* a_scales,
                   const uint8_t* w_codes, const uint8_t* w_scales, const float* bias, const float* ra, const float* rw,

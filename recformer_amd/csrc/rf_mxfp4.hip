@@ -5,7 +5,7 @@
 //              ties to the even one, above 6 to 6; a block of zeros: s = 0; a block with inf or NaN: s = 255,
 //              which stands for NaN
 //   product    C[m][n] = sum over blocks b of 2^(sa + sw - 254) sum over the block of a w, then
-//              * ra[m] col_scale * rw[n] (cosine scores) and + bias[n]
+//              * ra[m] col_scale * rw[n] (cosine scores; ra = rw = 1 without them) and + bias[n]
 //
 // Layout: codes (rows, KB 16) bytes, the even element in the low half of a byte; scales (rows, KB) bytes; KB =
 // ceil(K / 32), values past K are zero. Both contiguous. That is 4.25 bits a value: a 1M x 768 catalog is
@@ -181,7 +181,7 @@ __device__ __forceinline__ Cols cols_of(const MxArgs& a, int64_t n) {
   return {load_cols<true>(a.rw, n, a.N, 1.f), load_cols<true>(a.bias, n, a.N, 0.f)};
 }
 
-// four consecutive columns of row m: (v * ra * rw) + bias, rounded once (without ra: ra = rw = 1, exact)
+// four consecutive columns of row m: (v * ra * rw) + bias, rounded once; ra: the row's factor times col_scale
 template <typename T>
 __device__ __forceinline__ void store4(const MxArgs& a, int64_t m, int64_t n, f32x4 v, float ra, const Cols& c) {
   T* o = (T*)a.c + m * a.ldc + n;
@@ -256,14 +256,13 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, int64_t mw, int64_t
                                             const f32x4 (&acc)[4][4], const MxVec<T>& vec) {
   constexpr int NV = MxVec<T>::NV, NQ = MxVec<T>::NQ;
   const bool odd = r & 1;
-  const float scale = a.ra ? a.col_scale : 1.f;
   const int row = (int)a.ldc * (int)sizeof(T);
   const int at = (r & ~1) * row + (NV * g + (odd ? 4 * NV : 0)) * (int)sizeof(T);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
         (T*)a.c + (mw + j * 16) * a.ldc + nw, (short)0, 0x7FFFFFFF, 0x00020000);
-    const float ra = vec.ra[j] * scale;
+    const float ra = vec.ra[j] * a.col_scale;
 #pragma unroll
     for (int q = 0; q < NQ; q += 2) {
       u32x4 w[2];
@@ -624,7 +623,7 @@ __global__ void __launch_bounds__(256) k_mxfp4_skinny(MxArgs a) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       const int64_t m = (int64_t)j * 16 + r;
-      if (m < a.M) store4<T>(a, m, n, acc[i][j], a.ra ? a.ra[m] * a.col_scale : 1.f, c);
+      if (m < a.M) store4<T>(a, m, n, acc[i][j], (a.ra ? a.ra[m] : 1.f) * a.col_scale, c);
     }
   }
 }

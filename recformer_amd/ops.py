@@ -1258,7 +1258,8 @@ def mxfp4_gemm(a, w: Mxfp4, bias: Optional[torch.Tensor] = None, out_dtype: Opti
                ra: Optional[torch.Tensor] = None, rw: Optional[torch.Tensor] = None, col_scale: float = 1.0,
                tag: Optional[str] = None) -> torch.Tensor:
     """rf_mxfp4_gemm: C = a . w^T on the 4-bit matrix cores, fp32 sums, * ra[m] col_scale * rw[n] (cosine scores,
-    as gemm's RF_EPI_COS) and + bias[n], rounded once to out_dtype (default: a's type, fp32 for an Mxfp4). a:
+    as gemm's RF_EPI_COS; without ra and rw only * col_scale) and + bias[n], rounded once to out_dtype (default: a's
+    type, fp32 for an Mxfp4). a:
     (M, K) rows, quantised on the way, or an Mxfp4. The (M, N) result's rows are padded to 128 bytes."""
     lib = _lib.load()
     if not isinstance(a, Mxfp4):

@@ -310,3 +310,20 @@ def test_empty_and_refused(dev):
         ops.mxfp4_quantize(x[:1].expand(3, 64))
     with pytest.raises(ValueError):
         Mxfp4Catalog(w, torch.ones(9, device=dev))
+
+
+@pytest.mark.parametrize("M,N", [(1, 40), (5, 33001), (64, 32900), (90, 70), (200, 300)])
+def test_scale_without_row_and_column_factors(dev, M, N):
+    """col_scale alone: a power of two is exact, with a bias the sum is rounded once more."""
+    a = ops.mxfp4_quantize(rows_of(dev, torch.bfloat16, M, 96, 1))
+    w = ops.mxfp4_quantize(rows_of(dev, torch.bfloat16, N, 96, 2))
+    bias = torch.randn(N, device=dev)
+    c = ops.mxfp4_gemm(a, w)
+    assert torch.equal(ops.mxfp4_gemm(a, w, col_scale=0.25), c * 0.25)
+    want = c.double() * 0.25 + bias.double()
+    d = (ops.mxfp4_gemm(a, w, bias, col_scale=0.25).double() - want).abs()
+    assert bool((d <= U * want.abs()).all())
+    ones = torch.ones(max(M, N), device=dev)
+    for out in DTYPES:  # factors of 1 change nothing
+        assert torch.equal(ops.mxfp4_gemm(a, w, bias, out, col_scale=0.3),
+                           ops.mxfp4_gemm(a, w, bias, out, ones[:M], ones[:N], 0.3))
