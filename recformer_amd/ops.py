@@ -1096,6 +1096,8 @@ def token_logprobs_bwd(logits: torch.Tensor, stats: torch.Tensor, tokens: Option
     M = rows[1]
     f32 = torch.float32
     ids, C = None, 0
+    if tokens is None and g_logp is not None:
+        raise ValueError("token_logprobs_bwd: g_logp without the tokens it belongs to")
     if tokens is not None and g_logp is not None:
         if g_logp.shape != tokens.shape:
             raise ValueError(f"token_logprobs_bwd: g_logp {tuple(g_logp.shape)} for tokens {tuple(tokens.shape)}")
@@ -1259,8 +1261,8 @@ def mxfp4_gemm(a, w: Mxfp4, bias: Optional[torch.Tensor] = None, out_dtype: Opti
                tag: Optional[str] = None) -> torch.Tensor:
     """rf_mxfp4_gemm: C = a . w^T on the 4-bit matrix cores, fp32 sums, * ra[m] col_scale * rw[n] (cosine scores,
     as gemm's RF_EPI_COS; without ra and rw only * col_scale) and + bias[n], rounded once to out_dtype (default: a's
-    type, fp32 for an Mxfp4). a:
-    (M, K) rows, quantised on the way, or an Mxfp4. The (M, N) result's rows are padded to 128 bytes."""
+    type, fp32 for an Mxfp4). a: (M, K) rows, quantised on the way, or an Mxfp4. The (M, N) result's rows are padded
+    to 128 bytes."""
     lib = _lib.load()
     if not isinstance(a, Mxfp4):
         out_dtype = out_dtype or a.dtype

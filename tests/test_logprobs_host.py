@@ -248,3 +248,15 @@ def test_product_tiles_are_counted_in_64_bits():
     for M in (2 ** 31 - 127, 2 ** 31 - 1):
         assert "too many tiles" in err(lib.rf_mxfp4_gemm(0, M, 1 << 24, 32, A, A, A, A, None, None, None, 1.0, A, 1 << 24,
                                                          None))
+
+
+def test_weights_without_their_tokens_are_refused(monkeypatch):
+    """Without tokens the log probabilities' weights would be left out of the gradient."""
+    monkeypatch.setattr(ops, "_dev", lambda *ts: None)
+    monkeypatch.setattr(ops, "_logprobs_grad", lambda *a: a)
+    x, stats, g = torch.zeros(2, 8), torch.zeros(2, 4), torch.ones(2)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.token_logprobs_bwd(x, stats, None, g)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.token_logprobs_bwd(x, stats, None, g, g, g)
+    ops.token_logprobs_bwd(x, stats, None, None, g, g)
