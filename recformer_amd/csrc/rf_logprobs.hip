@@ -721,12 +721,13 @@ __global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __re
       ca = fmaf(cb, a.entropy[r], ca);
     }
   }
-  const float k1 = empty ? 0.f : a.it * rs;
   const float lrs = empty ? 0.f : __builtin_amdgcn_logf(rs) * LP_LN2;  // -ln s
+  // the gradient over it: the temperature comes last, since it c alone may be past fp32's range (0 * inf in the
+  // columns of p = 0, inf - inf where the weights of a listed entry and of p cancel)
   auto grad = [&](float v) {
     const float u = (v - m) * a.c2;
     const float c = ENT ? fmaf(cb, fmaf(fmaxf(u, -200.f), LP_LN2, lrs), ca) : ca;
-    return __builtin_amdgcn_exp2f(u) * (k1 * c);
+    return __builtin_amdgcn_exp2f(u) * (rs * c);
   };
 #pragma unroll
   for (int i = 0; i < LB_R; ++i) {
@@ -735,7 +736,7 @@ __global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __re
       const int64_t c0 = (int64_t)(j0 + j) * V - off;
       T o[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = from_f32<T>(empty ? 0.f : grad(Row<T>::at(raw[i], e)));
+      for (int e = 0; e < V; ++e) o[e] = from_f32<T>(empty ? 0.f : a.it * grad(Row<T>::at(raw[i], e)));
       if (c0 >= 0 && c0 + V <= a.N) {
         u32x4 w;
         __builtin_memcpy(&w, o, 16);
@@ -761,7 +762,7 @@ __global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __re
         head &= i >= j;
         w += sw[i];
       }
-    if (head) dx[id] = from_f32<T>(fmaf(a.it, w, grad(to_f32(x[id]))));
+    if (head) dx[id] = from_f32<T>(a.it * (w + grad(to_f32(x[id]))));
   }
 }
 

@@ -582,3 +582,23 @@ def test_saved_tensor_hooks_that_move_the_lists(dev, N):
             out = fn(leaf)
         got, = torch.autograd.grad(out, leaf)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [40, 5000, 100000])
+def test_gradient_at_inverse_temperatures_next_to_the_largest(dev, dt, N):
+    """it = 1e38 and weights that sum to 6: it times their sum is past fp32's range, every gradient is within it: 0
+    where p = 0 and nothing is listed, +-2e38 at the listed entries."""
+    x = logits_of(dev, dt, 3, N, N)
+    x[:, N // 2] = 40.0
+    tokens = torch.tensor([[N // 2, N // 2, 1]] * 3, device=dev)
+    w, wh = torch.full((3, 3), 2.0, device=dev), torch.ones(3, device=dev)
+    leaf = x.clone().requires_grad_()
+    logp, h = train.token_logprobs_train(leaf, tokens, inv_temp=1e38)
+    both, = torch.autograd.grad((logp, h), leaf, (w, wh), retain_graph=True)
+    only, = torch.autograd.grad(logp, leaf, w)
+    for d, gh in ((both, wh), (only, torch.zeros_like(wh))):
+        want, size = ref_grad(x, 1e38, tokens, w, gh)
+        assert float(want.abs().max()) < 2.1e38 and bool((want != 0).sum(1).eq(2).all())
+        close_grad(d, want, size)
+        assert int((d != 0).sum()) == 6
