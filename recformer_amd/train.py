@@ -604,9 +604,10 @@ def topk_distill_train(logits: torch.Tensor, teacher_logits: torch.Tensor, teach
                        temp: float = 1.0) -> torch.Tensor:
     """Distillation loss (scalar, fp32): temp^2 * mean over the rows that list something of KL(q || p), with
     q = softmax(teacher_logits / temp) over teacher_ids and p = softmax(logits / temp) over every column
-    (ops.topk_distill). The factor keeps the gradient's size independent of temp."""
-    if not temp > 0:
-        raise ValueError(f"topk_distill_train: temperature {temp} must be positive")
+    (ops.topk_distill). The factor keeps the gradient's size independent of temp; temp is within 1e-18 to 1e18, so
+    that temp^2 is within fp32's range."""
+    if not 1e-18 <= temp <= 1e18:
+        raise ValueError(f"topk_distill_train: temperature {temp} must be within 1e-18 to 1e18")
     return _TopkDistill.apply(logits, teacher_logits, teacher_ids, float(temp))
 
 

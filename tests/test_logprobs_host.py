@@ -260,3 +260,15 @@ def test_weights_without_their_tokens_are_refused(monkeypatch):
     with pytest.raises(ValueError, match="tokens"):
         ops.token_logprobs_bwd(x, stats, None, g, g, g)
     ops.token_logprobs_bwd(x, stats, None, None, g, g)
+
+
+def test_temperatures_whose_square_leaves_fp32_are_refused(monkeypatch):
+    """temp^2 is 0 or inf there: a loss and gradient of 0, or NaN."""
+    monkeypatch.setattr(train._TopkDistill, "apply", lambda *a: a[-1])
+    x, ids = torch.zeros(2, 8), torch.zeros(2, 1, dtype=torch.long)
+    for bad in (1e-30, 9e-19, 1.1e18, 1e20, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            train.topk_distill_train(x, x[:, :1], ids, bad)
+    for temp in (1e-18, 1, 2.5, 1e18):
+        assert train.topk_distill_train(x, x[:, :1], ids, temp) == temp
+        assert 0 < ctypes.c_float(temp * temp).value < float("inf")
