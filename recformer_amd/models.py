@@ -811,7 +811,8 @@ class RecformerForSeqRec(nn.Module):
                 raise ValueError(f"item_logprobs: seen {tuple(seen.shape)} for {B} users: (B, S)")
             # amin: a slot that leaves out nothing leaves its column as it is, whatever another slot says of it
             none = (seen < 0) | (seen >= N)
-            mask = torch.full(seen.shape, float("-inf"), device=scores.device).masked_fill_(none, float("inf"))
+            mask = torch.full(seen.shape, float("-inf"), dtype=scores.dtype, device=scores.device)
+            mask.masked_fill_(none, float("inf"))
             scores = scores.scatter_reduce(1, seen.to(torch.int64).clamp(0, N - 1), mask, "amin")
         return ops.token_logprobs(scores, items, k=k, want_entropy=want_entropy)
 

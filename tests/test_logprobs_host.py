@@ -272,3 +272,30 @@ def test_temperatures_whose_square_leaves_fp32_are_refused(monkeypatch):
     for temp in (1e-18, 1, 2.5, 1e18):
         assert train.topk_distill_train(x, x[:, :1], ids, temp) == temp
         assert 0 < ctypes.c_float(temp * temp).value < float("inf")
+
+
+class Scorer:
+    """The scores of 2 users and 6 items in the place of a model's."""
+
+    def similarity_score(self, z):
+        return torch.arange(12, dtype=torch.float32).view(2, 6)
+
+
+@pytest.fixture
+def masked_scores(monkeypatch):
+    from recformer_amd.models import RecformerForSeqRec
+    monkeypatch.setattr(ops, "token_logprobs", lambda scores, *a, **kw: scores)
+    return lambda seen: RecformerForSeqRec.item_logprobs(Scorer(), None, seen=seen)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16])
+def test_history_under_another_default_type(masked_scores, dtype):
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        got = masked_scores(torch.tensor([[5, -1], [0, 0]]))
+    finally:
+        torch.set_default_dtype(was)
+    want = Scorer().similarity_score(None)
+    want[0, 5] = want[1, 0] = -float("inf")
+    assert got.dtype == torch.float32 and torch.equal(got, want)
