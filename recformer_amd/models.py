@@ -809,6 +809,8 @@ class RecformerForSeqRec(nn.Module):
             B, N = scores.shape
             if seen.dim() != 2 or seen.shape[0] != B:
                 raise ValueError(f"item_logprobs: seen {tuple(seen.shape)} for {B} users: (B, S)")
+            if seen.dtype == torch.bool or seen.is_floating_point() or seen.is_complex():
+                raise TypeError(f"item_logprobs: seen are item ids, got {seen.dtype}")
             # amin: a slot that leaves out nothing leaves its column as it is, whatever another slot says of it
             none = (seen < 0) | (seen >= N)
             mask = torch.full(seen.shape, float("-inf"), dtype=scores.dtype, device=scores.device)

@@ -299,3 +299,12 @@ def test_history_under_another_default_type(masked_scores, dtype):
     want = Scorer().similarity_score(None)
     want[0, 5] = want[1, 0] = -float("inf")
     assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+def test_history_that_is_no_list_of_ids_is_refused(masked_scores):
+    """A mask over the items would be taken for the ids 0 and 1, and fractions would be cut."""
+    for seen in (torch.ones(2, 6, dtype=torch.bool), torch.ones(2, 1), torch.ones(2, 1, dtype=torch.bfloat16)):
+        with pytest.raises(TypeError):
+            masked_scores(seen)
+    for dtype in (torch.uint8, torch.int16, torch.int32, torch.int64):
+        assert bool(torch.isneginf(masked_scores(torch.tensor([[5], [0]], dtype=dtype))[[0, 1], [5, 0]]).all())
