@@ -811,11 +811,12 @@ class RecformerForSeqRec(nn.Module):
                 raise ValueError(f"item_logprobs: seen {tuple(seen.shape)} for {B} users: (B, S)")
             if seen.dtype == torch.bool or seen.is_floating_point() or seen.is_complex():
                 raise TypeError(f"item_logprobs: seen are item ids, got {seen.dtype}")
+            seen = seen.to(torch.int64)  # (N may not fit a narrower type, and would be cut in the comparison)
             # amin: a slot that leaves out nothing leaves its column as it is, whatever another slot says of it
             none = (seen < 0) | (seen >= N)
             mask = torch.full(seen.shape, float("-inf"), dtype=scores.dtype, device=scores.device)
             mask.masked_fill_(none, float("inf"))
-            scores = scores.scatter_reduce(1, seen.to(torch.int64).clamp(0, N - 1), mask, "amin")
+            scores = scores.scatter_reduce(1, seen.clamp(0, N - 1), mask, "amin")
         return ops.token_logprobs(scores, items, k=k, want_entropy=want_entropy)
 
     def distill_loss(self, teacher_logits, teacher_ids, distill_temp: float = 1.0, **batch):

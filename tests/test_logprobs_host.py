@@ -308,3 +308,10 @@ def test_history_that_is_no_list_of_ids_is_refused(masked_scores):
             masked_scores(seen)
     for dtype in (torch.uint8, torch.int16, torch.int32, torch.int64):
         assert bool(torch.isneginf(masked_scores(torch.tensor([[5], [0]], dtype=dtype))[[0, 1], [5, 0]]).all())
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.uint8, 10000), (torch.int8, 200), (torch.int16, 50265)])
+def test_history_ids_of_a_type_narrower_than_the_catalog(masked_scores, monkeypatch, dtype, n):
+    monkeypatch.setattr(Scorer, "similarity_score", lambda self, z: torch.zeros(2, n))
+    got = masked_scores(torch.tensor([[100, 3], [0, 127]], dtype=dtype))
+    assert torch.isneginf(got).nonzero().tolist() == [[0, 3], [0, 100], [1, 0], [1, 127]]
