@@ -327,3 +327,49 @@ def test_scale_without_row_and_column_factors(dev, M, N):
     for out in DTYPES:  # factors of 1 change nothing
         assert torch.equal(ops.mxfp4_gemm(a, w, bias, out, col_scale=0.3),
                            ops.mxfp4_gemm(a, w, bias, out, ones[:M], ones[:N], 0.3))
+
+
+def _at_any_byte(q):
+    """q with its scales one byte off a word's border."""
+    buf = torch.empty(q.scales.numel() + 8, dtype=torch.uint8, device=q.scales.device)
+    s = buf[1:1 + q.scales.numel()].view(q.scales.shape)
+    s.copy_(q.scales)
+    return ops.Mxfp4(q.codes, s, q.k)
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("K", [96, 256, 512, 768, 800])
+def test_product_of_several_tiles_a_workgroup(dev, out, K, aligned):
+    """33 x 40 tiles, more than two for each workgroup there is, whole ones and those of an edge after one another,
+    one to four steps of K each, different numbers in every row: the tile's limits as in test_product."""
+    M, N = 4200, 5000
+    a = ops.mxfp4_quantize(rows_of(dev, torch.float32, M, K, 1))
+    w = ops.mxfp4_quantize(rows_of(dev, torch.bfloat16, N, K, 2) * 0.01)
+    if not aligned:
+        a, w = _at_any_byte(a), _at_any_byte(w)
+    va, vw = ref_values(a), ref_values(w)
+    want, size = va @ vw.t(), va.abs() @ vw.abs().t()
+    g = torch.Generator(device=dev).manual_seed(3)
+    bias = torch.randn(N, device=dev, generator=g)
+    ra, rw = torch.rand(M, device=dev, generator=g) + 0.5, torch.rand(N, device=dev, generator=g) + 0.5
+
+    def close(got, ref, sz):
+        lim = (K + 4) * U * sz + torch.finfo(out).eps / 2 * ref.abs() + torch.finfo(out).smallest_normal * 2 ** -10
+        keep = ref.abs() + lim < torch.finfo(out).max
+        assert got.dtype == out
+        d = (got.double() - ref).abs()
+        assert bool((d <= lim)[keep].all()), float((d - lim)[keep].max())
+        assert bool(keep.float().mean() > 0.99)
+
+    close(ops.mxfp4_gemm(a, w, out_dtype=out), want, size)
+    close(ops.mxfp4_gemm(a, w, bias, out), want + bias.double(), size + bias.double().abs())
+    f = ra.double()[:, None] * rw.double() * 0.05
+    close(ops.mxfp4_gemm(a, w, None, out, ra, rw, 0.05), want * f, size * f)
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(2, 33000, 64), (5, 32769, 256), (16, 33001, 160), (16, 32770, 1600), (32, 33003, 128),
+                                   (17, 40007, 33), (64, 32800, 512), (40, 50265, 768), (64, 33000, 1056)])
+def test_product_of_few_rows_and_many_columns_in_16_bits(dev, out, M, N, K):
+    test_product(dev, out, M, N, K)
