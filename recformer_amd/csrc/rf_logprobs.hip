@@ -724,10 +724,11 @@ __global__ void __launch_bounds__(TPB) k_logprobs_bwd(LpBwdArgs a, const T* __re
   const float lrs = empty ? 0.f : __builtin_amdgcn_logf(rs) * LP_LN2;  // -ln s
   // the gradient over it: the temperature comes last, since it c alone may be past fp32's range (0 * inf in the
   // columns of p = 0, inf - inf where the weights of a listed entry and of p cancel)
+  ca *= rs;
+  cb *= rs;
   auto grad = [&](float v) {
     const float u = (v - m) * a.c2;
-    const float c = ENT ? fmaf(cb, fmaf(fmaxf(u, -200.f), LP_LN2, lrs), ca) : ca;
-    return __builtin_amdgcn_exp2f(u) * (rs * c);
+    return __builtin_amdgcn_exp2f(u) * (ENT ? fmaf(cb, fmaf(fmaxf(u, -200.f), LP_LN2, lrs), ca) : ca);
   };
 #pragma unroll
   for (int i = 0; i < LB_R; ++i) {
