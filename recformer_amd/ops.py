@@ -1175,15 +1175,15 @@ def topk_distill_bwd(logits: torch.Tensor, stats: torch.Tensor, teacher_logits: 
     for t in (g, coef):
         if t.numel() != 1 or t.dtype != torch.float32 or t.get_device() != logits.get_device():
             raise ValueError("topk_distill_bwd: g and coef are one-element fp32 tensors beside the logits")
-    return _distill_grad(rows, logits, stats.data_ptr(), val, ids, g, coef.data_ptr())
+    return _distill_grad(rows, logits, stats.data_ptr(), val, ids, ids.shape[1], g, coef.data_ptr())
 
 
-def _distill_grad(rows, logits, stats: int, val, ids, g, coef: int) -> torch.Tensor:
-    """The checked call; rows: _logit_rows of these logits, val and ids as _teacher gives them, stats and coef
-    addresses."""
+def _distill_grad(rows, logits, stats: int, val, ids, K: int, g, coef: int) -> torch.Tensor:
+    """The checked call; rows: _logit_rows of these logits, val and ids of K entries a row as _teacher gives them, stats
+    and coef addresses."""
     out, ldd = _like_rows(rows, logits)
-    _run(_lib.load().rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, *rows, stats, val.data_ptr(), ids.data_ptr(),
-         ids.shape[1], g.data_ptr(), coef, out.data_ptr(), ldd)
+    _run(_lib.load().rf_topk_distill_bwd, "rf_topk_distill_bwd", logits, *rows, stats, val.data_ptr(), ids.data_ptr(), K,
+         g.data_ptr(), coef, out.data_ptr(), ldd)
     return out
 
 
@@ -1202,33 +1202,29 @@ class Mxfp4(NamedTuple):
         return self.codes.shape[0]
 
 
-def _mxfp4_size(what: str, rows: int, k: int) -> None:
-    """What the entry points take in their C ints."""
-    if rows >= 2 ** 31 or not 1 <= k <= 2 ** 24:
-        raise ValueError(f"{what}: {rows} rows of {k} values (fewer than 2^31 rows, 1 to 2^24 values)")
-
-
 def _mxfp4_check(what: str, q: Mxfp4) -> None:
-    _mxfp4_size(what, q.codes.shape[0], q.k)
     _dev(q.codes, q.scales)
-    kb = (q.k + 31) // 32
+    rows, k = q.codes.shape[0], q.k
+    kb = (k + 31) // 32
+    if rows >= 2 ** 31 or not 1 <= k <= 2 ** 24:  # what the entry points take in their C ints
+        raise ValueError(f"{what}: {rows} rows of {k} values: fewer than 2^31 rows, 1 to 2^24 values")
     for t, name, w in ((q.codes, "codes", kb * 16), (q.scales, "scales", kb)):
-        if t.dtype != torch.uint8 or t.dim() != 2 or tuple(t.shape) != (q.codes.shape[0], w) or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} for k={q.k}: contiguous uint8 (rows, {w})")
+        if t.dtype != torch.uint8 or t.dim() != 2 or tuple(t.shape) != (rows, w) or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} {t.dtype} for k={k}: contiguous uint8 (rows, {w})")
     if q.codes.data_ptr() % 16 or q.scales.device != q.codes.device:
         raise ValueError(f"{what}: codes must be 16-byte aligned, scales beside them")
 
 
 def _mxfp4_rows(x: torch.Tensor, want_rnorm: bool, eps: float):
     lib = _lib.load()
-    if x.dim() == 2:
-        _mxfp4_size("mxfp4_quantize", *x.shape)
     _dev(x)
     code = dtype_code(x.dtype)
     ld = _rowmajor(x, "x")
     M, K = x.shape
-    if M > 1 and ld < K:
+    if K < 1 or (M > 1 and ld < K):
         raise ValueError(f"mxfp4_quantize: rows of shape {tuple(x.shape)}, strides {x.stride()}")
+    if M >= 2 ** 31 or K > 2 ** 24:  # the entry points take C ints
+        raise ValueError(f"mxfp4_quantize: {M} rows of {K} values: fewer than 2^31 rows, 1 to 2^24 values")
     kb = (K + 31) // 32
     codes = torch.empty(M, kb * 16, dtype=torch.uint8, device=x.device)
     scales = torch.empty(M, kb, dtype=torch.uint8, device=x.device)

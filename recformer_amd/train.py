@@ -521,27 +521,28 @@ def _differentiable_once(backward):
     return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
-def _saved_again(ctx, logits, *lists):
-    """(the forward's ops._logit_rows, logits, lists) of the saved logits and of the lists and buffers beside them,
-    contiguous in the forward. Hooks on saved tensors may have moved them or changed their strides; what they left on
-    another device, or gave another type or shape, is refused before it reaches a kernel by its address."""
-    dev, layout, rows = ctx.layout[0], ctx.layout[1:], ctx.rows
-    for t, (dtype, shape) in zip((logits, *lists), layout):
-        if t.get_device() != dev or t.dtype != dtype or t.shape != shape:
-            raise ValueError(f"saved tensors: {tuple(t.shape)} {t.dtype} on {t.device} in the place of "
-                             f"{tuple(shape)} {dtype} of the forward's device")
+def _rows_again(ctx, logits):
+    """(the forward's ops._logit_rows, logits) of saved logits. Hooks on saved tensors may have moved them or changed
+    their strides; logits on another device, or of another type or shape, are refused before they reach a kernel by
+    their address."""
+    rows = ctx.rows
+    if logits.dtype != ctx.dtype or logits.shape != ctx.shape or logits.get_device() != ctx.dev:
+        raise ValueError(f"saved logits: {tuple(logits.shape)} {logits.dtype} on {logits.device} in the place of the "
+                         f"forward's {tuple(ctx.shape)} {ctx.dtype}")
     if logits.data_ptr() != rows[3] or logits.stride() != ctx.strides:
-        if logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]:
+        if logits.stride(1) != 1 or logits.stride(0) < rows[2]:
             logits = logits.contiguous()
         rows = ops._logit_rows("saved logits", logits, rows[-1])
-    return rows, logits, [t if t.is_contiguous() else t.contiguous() for t in lists]
+    return rows, logits
 
 
-def _save_rows(ctx, rows, logits, *lists):
-    """Saves the logits and the lists and buffers beside them for _saved_again; rows: ops._logit_rows of the logits."""
-    ctx.save_for_backward(logits, *lists)
-    ctx.rows, ctx.strides = rows, logits.stride()
-    ctx.layout = (logits.get_device(), *((t.dtype, t.shape) for t in (logits, *lists)))
+def _list_again(ctx, t, n: int, dtype=torch.float32):
+    """A saved list or buffer of n numbers beside the logits, contiguous as in the forward; refused where it is no such
+    list on the forward's device."""
+    if t.dtype != dtype or t.numel() != n or t.get_device() != ctx.dev:
+        raise ValueError(f"saved tensors: {tuple(t.shape)} {t.dtype} on {t.device} in the place of {n} numbers of "
+                         f"{dtype} beside the logits")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -554,8 +555,10 @@ class _TokenLogprobs(torch.autograd.Function):
         rows = ops._logit_rows("token_logprobs_train", logits, inv_temp)
         ids = ops._token_ids("token_logprobs_train: tokens", tokens, logits)
         r = ops._logprobs(rows, logits, ids, tokens.shape, 0, ignore_index, True, True)
-        _save_rows(ctx, rows, logits, ids, r.stats, r.entropy)
-        ctx.ignore = ignore_index
+        ctx.save_for_backward(logits, ids, r.stats, r.entropy)
+        ctx.rows, ctx.strides, ctx.shape, ctx.dtype, ctx.dev = (rows, logits.stride(), logits.shape, logits.dtype,
+                                                                logits.get_device())
+        ctx.C, ctx.ignore = ids.shape[1], ignore_index
         ctx.set_materialize_grads(False)
         return r.logp, r.entropy
 
@@ -564,12 +567,18 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, g_logp, g_entropy):
         if not ctx.needs_input_grad[0] or (g_logp is None and g_entropy is None):
             return None, None, None, None
-        rows, logits, (ids, stats, entropy) = _saved_again(ctx, *ctx.saved_tensors)
+        logits, ids, stats, entropy = ctx.saved_tensors
+        rows, logits = _rows_again(ctx, logits)
+        M, C = rows[1], ctx.C
+        ids = _list_again(ctx, ids, M * C, torch.int64)
+        stats = _list_again(ctx, stats, 4 * M)
+        entropy = _list_again(ctx, entropy, M)
         if g_logp is not None and not g_logp.is_contiguous():
             g_logp = g_logp.contiguous()
         if g_entropy is not None and not g_entropy.is_contiguous():
             g_entropy = g_entropy.contiguous()
-        C = 0 if g_logp is None else ids.shape[1]
+        if g_logp is None:
+            C = 0
         return ops._logprobs_grad(rows, logits, stats, ids, C, ctx.ignore, g_logp, entropy, g_entropy), None, None, None
 
 
@@ -582,7 +591,10 @@ class _TopkDistill(torch.autograd.Function):
         rows = ops._logit_rows("topk_distill_train", logits, 1.0 / temp)
         val, ids = ops._teacher("topk_distill_train", logits, teacher_logits, teacher_ids)
         loss, buf = ops._distill(rows, logits, val, ids, temp * temp)
-        _save_rows(ctx, rows, logits, val, ids, buf)
+        ctx.save_for_backward(logits, val, ids, buf)
+        ctx.rows, ctx.strides, ctx.shape, ctx.dtype, ctx.dev = (rows, logits.stride(), logits.shape, logits.dtype,
+                                                                logits.get_device())
+        ctx.K = ids.shape[1]
         return loss
 
     @staticmethod
@@ -590,9 +602,14 @@ class _TopkDistill(torch.autograd.Function):
     def backward(ctx, g):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
-        rows, logits, (val, ids, buf) = _saved_again(ctx, *ctx.saved_tensors)
+        logits, val, ids, buf = ctx.saved_tensors
+        rows, logits = _rows_again(ctx, logits)
+        M, K = rows[1], ctx.K
+        val = _list_again(ctx, val, M * K)
+        ids = _list_again(ctx, ids, M * K, torch.int64)
+        buf = _list_again(ctx, buf, 5 * M + 1)
         at = buf.data_ptr()
-        return ops._distill_grad(rows, logits, at, val, ids, g, at + 20 * rows[1]), None, None, None
+        return ops._distill_grad(rows, logits, at, val, ids, K, g, at + 20 * M), None, None, None
 
 
 def token_logprobs_train(logits: torch.Tensor, tokens: torch.Tensor, inv_temp: float = 1.0, ignore_index: int = -100):

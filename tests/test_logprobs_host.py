@@ -220,15 +220,20 @@ def test_saved_tensors_left_elsewhere_are_refused(monkeypatch, kind):
         back()
         assert len(calls) == 1
         for i, t in enumerate(saved):
-            for bad in (t.as_subclass(torch.Tensor), t.to(torch.float64), t[:-1], t.reshape(-1, 1, 1)):
+            for bad in (t.as_subclass(torch.Tensor), t.to(torch.float64), t[:-1], t.repeat_interleave(2)):
                 ctx.saved_tensors = saved[:i] + (bad,) + saved[i + 1:]
                 with pytest.raises(ValueError):
                     back()
+        for bad in (saved[0].t(), saved[0].reshape(6, 20), saved[0].reshape(3, 8, 5)):
+            ctx.saved_tensors = (bad, *saved[1:])
+            with pytest.raises(ValueError):
+                back()
     assert len(calls) == 1
 
 
-def test_mxfp4_sizes_past_the_c_ints_are_refused():
+def test_mxfp4_sizes_past_the_c_ints_are_refused(monkeypatch):
     """2^32 rows would be 0 rows there, 2^32 + 32 columns a row of 32: refused before anything is allocated."""
+    monkeypatch.setattr(ops, "_dev", lambda *ts: None)
     for rows, k in ((2 ** 31, 32), (2 ** 32, 32), (2 ** 32 + 3, 1), (1, 2 ** 24 + 1), (2, 2 ** 32 + 32)):
         x = torch.empty(rows, k, dtype=torch.bfloat16, device="meta")
         kb = -(-k // 32)
