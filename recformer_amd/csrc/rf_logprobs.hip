@@ -467,9 +467,12 @@ struct RowSrc {
 // ---- one slice of a row ------------------------------------------------------------------------
 // Loads, maximum, exponentials and alternatives follow one another within a workgroup; two of 1024 threads a CU
 // (64 registers) let one load while the other computes. Reading bounds it for fp32 (128 x 1M: 88 us, 5.8 TB/s);
-// 16-bit rows come within a tenth of that (4915 x 50265 bf16: 91 us, 5.4 TB/s), and what comes on top shows: the
-// entropy's two operations an element (108 us), the barriers and the one-wave search of the alternatives (top 20
-// 120 us, with the entropy 129, top 256 214; 128 x 1M fp32 top 50 110).
+// 16-bit rows come within a tenth or two of that (4915 x 50265 bf16: 98 us, 5.1 TB/s), and what comes on top shows:
+// the entropy's two operations an element (110 us), the barriers and the one-wave search of the alternatives (top 20
+// 130 us, with the entropy 133, top 256 216 and 224; 128 x 1M fp32 top 50 with the entropy 110). Launches one after
+// another over three inputs in turn.
+// With alternatives the 1024 threads' 64 registers do not hold it all: four of a thread's go to scratch memory, for
+// bf16 one of them in every thread, which writes 20 MB at 4915 x 50265 where the results are 1.3 MB.
 template <typename T, int TPB, bool ENT, bool TOP, bool TEACH>
 __global__ void __launch_bounds__(TPB, TPB == 1024 ? 8 : 4) k_logprobs(LpArgs a, const T* __restrict__ logits) {
   constexpr int V = Row<T>::V;
@@ -625,7 +628,7 @@ __global__ void __launch_bounds__(TPB) k_logprobs_join(LpArgs a, const T* __rest
 // ---- mean of the rows' losses over the rows that list something --------------------------------
 // loss = scale sum(rows) / n, coef = scale / n with n = #{r : 1 / teacher sum != 0}; one workgroup, so
 // the order of the sum is fixed (0 / 0 = NaN where no row lists anything, as the mean cross entropy has it). Latency:
-// 4.5 us for 4915 rows
+// 4.5 us for 4915 rows, and in proportion to M from there on (34 us for 100000, 311 for 1M)
 __global__ void __launch_bounds__(1024) k_rows_mean(int M, const float* __restrict__ rows,
                                                     const float* __restrict__ stats, float scale,
                                                     float* __restrict__ loss, float* __restrict__ coef) {
@@ -662,7 +665,7 @@ struct LpBwdArgs {
 
 // One slice of a row: read, e^t / s, write. The listed entries are then written again by one thread each
 // (after a barrier; the first of equal ids adds all their weights in list order), so nothing is added
-// atomically. HBM bound: 4915 x 50265 bf16 168 us (5.9 TB/s), 128 x 1M fp32 207 (4.9 TB/s); LB_R chunks a thread
+// atomically. HBM bound: 4915 x 50265 bf16 166 us (6.0 TB/s), 128 x 1M fp32 205 (5.0 TB/s); LB_R chunks a thread
 // keep enough loads in flight beside the stores.
 // PAST: the gradient is written past the caches.
 template <typename T, int TPB, bool ENT, bool PAST>

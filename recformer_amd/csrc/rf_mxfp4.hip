@@ -44,7 +44,7 @@ __device__ __forceinline__ void load8(const T* x, int c, int K, float (&v)[8]) {
 }
 
 // A row is taken by 2^sh lanes, eight values a lane at a time, four lanes a block. HBM bound (read the
-// row, write 17 bytes a block): 1M x 768 bf16 395 us, 4.9 TB/s, with the norms 432.
+// row, write 17 bytes a block): 1M x 768 bf16 361 us, 5.4 TB/s, with the norms 426.
 template <typename T>
 __global__ void __launch_bounds__(256) k_mxfp4_quantize(int64_t M, int K, int KB, const T* __restrict__ x, int64_t ldx,
                                                         int sh, float eps, uint8_t* __restrict__ codes,
@@ -95,7 +95,7 @@ __device__ __forceinline__ float scale_value(int s) {  // 2^(s - 127); 255: NaN
 }
 
 // Eights of values, flat over the rows (G = ceil(K / 8) a row), two a thread 64 apart so that a wave's loads and
-// stores are contiguous. HBM bound; the stores are non-temporal (1M x 768 to bf16: 318 us, 6.1 TB/s; 538 us
+// stores are contiguous. HBM bound; the stores are non-temporal (1M x 768 to bf16: 307 us, 6.3 TB/s; 538 us
 // through the caches). Rows of other alignments take unaligned stores (100000 x 770 bf16: 32 us; element by element
 // 100).
 template <typename T>
@@ -312,7 +312,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, int64_t mw, int64_t
 // epilogue); two workgroups a CU. W is the matrix instruction's first operand, so that a lane's results are
 // neighbours in a row of C; with 16-bit results the W rows of a pair of instructions are interleaved by fours,
 // so that a lane holds eight neighbours.
-// For short K the stores bound it (4096 x 125000 x 768 fp32: 413 us, 5.0 TB/s of results; 4915 x 50265 x 768 bf16 166 us,
+// For short K the stores bound it (4096 x 125000 x 768 fp32: 416 us, 4.9 TB/s of results; 4915 x 50265 x 768 bf16 167 us,
 // where stores alone take 108); for long K the fragments' and the LDS-DMA's way through LDS beside the matrix
 // instructions (8192^3: 376 us, 2.9 PFLOP/s). Loads two steps ahead, with a second barrier a step, took 5% longer.
 // Rows of a stage are 128 bytes; their 16-byte slots are permuted by three bits of the row, so that eight
@@ -527,9 +527,9 @@ __global__ void __launch_bounds__(256, 2) k_mxfp4_gemm(MxArgs a) {
 }
 
 // Up to 16 MT rows of A: W is read once from memory straight into the fragments, a wave per 16 NT of its rows,
-// U steps of K in flight; the A rows come from the caches. Bound by the read of W for few rows (1 x 1M x 768 88 us,
-// 4.7 TB/s; 1 x 100000 x 4096 41 us, 5.3 TB/s), by the A fragments' way through the caches for many (64 x 1M x 768
-// 231 us, 2.9 TB/s with the result). DW: a row's four scales of
+// U steps of K in flight; the A rows come from the caches. Bound by the read of W for few rows (two tables in turn:
+// 1 x 1M x 768 79 us, 5.2 TB/s; 1 x 100000 x 4096 48 us, 4.5 TB/s), by the A fragments' way through the caches for
+// many (16 x 1M x 768 110 us, 4.3 TB/s with the result, 64 x 1M x 768 210 us, 3.2 TB/s). DW: a row's four scales of
 // a step are an aligned word; the four lanes of a row load the words of four steps and trade them (a byte a lane and
 // step took 66 instead of 41 us at 1 x 100000 x 4096). Without, a lane loads its bytes (unaligned words took 100
 // instead of 92 us at 1 x 1M x 736).
